@@ -480,6 +480,111 @@ int rt_rope_kv_append_bf16(void* q, const void* k_in, const void* v_in, void* k_
                            const float* inv_freq, int64_t batch, int n_heads, int n_kv, int head_dim,
                            int64_t max_seq, int64_t pos, const int32_t* positions, int rope_style, void* stream);
 
+/* ===================================================================================== *
+ * A KV cache held in 4 bits (no counterpart in the reference).
+ *
+ * A row (one token of one KV head, K or V, D = 64, 128 or 256 values) is D codes of 4 bits and D/32 groups of
+ * 32 values with a scale and a minimum each: 5 bits a value.  With W = min(D, 128), value d belongs to group
+ *     (d / W) * (W / 32)  +  (d % (W / 4)) / 8,
+ * i.e. a group takes one run of 8 from every quarter of a span of W values (at D = 64 and 128 both values of a
+ * half-split rotary pair are in one group).  For the values x of a group, clamped to +-65504,
+ *     lo = fp16(min x),  scale = fp16(max(max x - lo, 0) / 15),  code = clamp(rint((x - lo) / scale), 0, 15)
+ * in f32 arithmetic (scale = 0: code 0), and the code stands for lo + scale * code.  A group with a NaN has
+ * lo = NaN, scale 0: all of it reads as NaN.
+ *   codes  : u8   [B,Hkv,max_seq,D/2], byte i = code 2i | code 2i+1 << 4
+ *   scales : fp16 [B,Hkv,max_seq,D/32,2], {scale, lo} of each group
+ * All four planes 16-byte aligned.
+ * ===================================================================================== */
+
+/*
+ * Quantises new rows into the cache: row i < lens[b] of sequence b goes to position positions[b] + i.
+ *   k, v       : bf16 [B,Hkv,rows,D] with element strides {batch, head, row} in k_strides, v_strides (HOST
+ *                pointers, NULL = contiguous), multiples of 8, the head dim contiguous, 16-byte aligned:
+ *                a projection's [B,T,Hkv*D] needs no transpose.  rows = 1 is a decode step's append.
+ *   positions  : device int32 [B], or NULL to start at `pos` in every sequence (then pos + rows <= max_seq);
+ *                rows that a device position puts outside the cache are dropped.
+ *   lens       : NULL or device int32 [B], rows of a padded batch that count.
+ */
+int rt_kv4_append(void* k_codes, void* k_scales, void* v_codes, void* v_scales, const void* k, const void* v,
+                  const int64_t* k_strides, const int64_t* v_strides, int64_t batch, int n_kv, int64_t rows,
+                  int head_dim, int64_t max_seq, int64_t pos, const int32_t* positions, const int32_t* lens,
+                  void* stream);
+
+/*
+ * rt_rope_kv_append_bf16 on a 4-bit cache, one launch: rotates q in place, and quantises the rotated K row
+ * (rounded to bf16 first, so that it is the row the bf16 cache would hold) and the V row into the cache.
+ *   positions / pos : the rotary position of each sequence;  slots / slot : the row of the cache that is written,
+ *   where it is another one (a cache that tokens were evicted from): slots a device int32 [B] or NULL,
+ *   slot < 0 and slots = NULL: the position.  A slot outside the cache, or a negative position, leaves the
+ *   sequence's q and cache as they were.
+ */
+int rt_rope_kv4_append(void* q, const void* k_in, const void* v_in, void* k_codes, void* k_scales, void* v_codes,
+                       void* v_scales, const float* inv_freq, int64_t batch, int n_heads, int n_kv, int head_dim,
+                       int64_t max_seq, int64_t pos, const int32_t* positions, int64_t slot, const int32_t* slots,
+                       int rope_style, void* stream);
+
+/*
+ * Rows of a 4-bit cache in bf16: k_out, v_out bf16 [B,Hkv,rows,D], row i is the cache's row starts[b] + i, or zero
+ * from min(kv_lens[b], max_seq) on (and in front of the cache).  What rt_attn_prefill_gqa_bf16 attends to for a
+ * chunk of a prompt.
+ *   starts : NULL or device int32 [B] (NULL: `start` for every sequence);  kv_lens : NULL (= max_seq) or device int32 [B].
+ */
+int rt_kv4_read(const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales, void* k_out,
+                void* v_out, int64_t batch, int n_kv, int head_dim, int64_t max_seq, int64_t rows, int64_t start,
+                const int32_t* starts, const int32_t* kv_lens, void* stream);
+
+/* Bytes of device scratch that rt_kv4_decode needs (weighed: with `weights`). */
+size_t rt_kv4_decode_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int head_dim, int64_t max_seq,
+                                     int weighed);
+
+/*
+ * Batched single-token GQA decode over a 4-bit cache: softmax(scale * q K^T) V of the values the codes stand for.
+ *   q, out : bf16 [B,Hq,D];  lse : NULL or f32 [B,Hq];  kv_lens : device int32 [B] (clamped to max_seq), or NULL
+ *   for kv_len_uniform;  scale <= 0 selects 1/sqrt(D).  Hq/Hkv from 1 to 8.  A sequence of length 0 gives
+ *   out = 0, lse = -inf.
+ *   weights : NULL or f32 [B,Hkv,max_seq]; weights[b,h,t] += the sum over the query heads of KV head h of the
+ *   softmax weight of token t < kv_len (what rt_kv_evict chooses by).
+ */
+int rt_kv4_decode(const void* q, const void* k_codes, const void* k_scales, const void* v_codes, const void* v_scales,
+                  void* out, float* lse, float* weights, int64_t batch, int64_t n_heads, int64_t n_kv_heads,
+                  int head_dim, int64_t max_seq, const int32_t* kv_lens, int64_t kv_len_uniform, float scale,
+                  void* workspace, size_t workspace_bytes, void* stream);
+
+/* ===================================================================================== *
+ * Eviction from a KV cache by accumulated attention weight (no counterpart in the reference).
+ * ===================================================================================== */
+
+/*
+ * Adds the softmax weights of queries over a bf16 cache to an accumulator:
+ *   weights[b,h,t] += sum over query heads g of KV head h and queries i of exp(scale * q[b,g,i] . k[b,h,t] - lse[b,g,i])
+ * for the t < kv_len that query i sees: the seq_q queries are the last ones of the sequence, query i sits at position
+ * kv_len - seq_q + i and sees the tokens up to its own (seq_q = 1: all of them).
+ *   q : bf16 [B,Hq,seq_q,D];  lse : f32 [B,Hq,seq_q] as the attention of the same queries returned it (a row with
+ *   lse = -inf adds nothing);  k_cache : bf16 [B,Hkv,max_seq,D], D = 64, 128 or 256;  weights : f32 [B,Hkv,max_seq].
+ *   Hq/Hkv from 1 to 8.  Deterministic: every weight has one writer.
+ */
+int rt_kv_weigh_bf16(const void* q, const void* k_cache, const float* lse, float* weights, int64_t batch,
+                     int64_t n_heads, int64_t n_kv_heads, int64_t seq_q, int head_dim, int64_t max_seq,
+                     const int32_t* kv_lens, int64_t kv_len_uniform, float scale, void* stream);
+
+/*
+ * Keeps `keep` rows of every (sequence, KV head) of a cache: the last `recent` ones and, of the others, those with
+ * the largest weights (of equal ones the first; a NaN counts as the largest).  They are written to the front of
+ * another cache in their order; a sequence of up to `keep` rows is copied.  Rows behind what is kept are left as
+ * they were.
+ *   n_planes (1 to 4) pairs of planes src[i] [B,Hkv,max_seq,row_bytes[i]] -> dst[i] [B,Hkv,max_seq_out,row_bytes[i]]:
+ *       K and V of a bf16 cache, or the four planes of a 4-bit one; HOST arrays; row_bytes multiples of 8, up to
+ *       4096; planes 16-byte aligned and none of src overlapping one of dst (nor weights weights_out, nor kv_lens lens_out).
+ *   weights : f32 [B,Hkv,max_seq];  weights_out : f32 [B,Hkv,max_seq_out], the kept rows' weights, zero behind them.
+ *   kept    : int32 [B,Hkv,keep], the rows' places in the source, -1 behind them;
+ *   lens_out : int32 [B], min(kv_len, keep).
+ *   0 <= recent <= keep <= max_seq_out, keep >= 1.  kv_lens / kv_len_uniform as in rt_kv4_decode.
+ */
+int rt_kv_evict(const void* const* src, void* const* dst, const int32_t* row_bytes, int n_planes, const float* weights,
+                float* weights_out, int32_t* kept, int32_t* lens_out, int64_t batch, int64_t n_kv_heads,
+                int64_t max_seq, int64_t max_seq_out, const int32_t* kv_lens, int64_t kv_len_uniform, int64_t keep,
+                int64_t recent, void* stream);
+
 /* f32 <-> bf16 (RNE) conversion of n elements on the device; helpers of the host entries. */
 int rt_convert_f32_to_bf16(const float* src, void* dst, int64_t n, void* stream);
 int rt_convert_bf16_to_f32(const void* src, float* dst, int64_t n, void* stream);

@@ -103,6 +103,30 @@ extern "C" {
         workspace_bytes: usize, stream: *mut c_void) -> c_int;
     pub fn rt_attn_merge_ll_rows(local_words: *const c_void, epoch: u32, wait_clocks: i64, world: c_int, rows: i64,
         dim: c_int, out_bf16: *mut c_void, out_f32: *mut f32, lse: *mut f32, stream: *mut c_void) -> c_int;
+    pub fn rt_kv4_append(k_codes: *mut c_void, k_scales: *mut c_void, v_codes: *mut c_void, v_scales: *mut c_void,
+        k: *const c_void, v: *const c_void, k_strides: *const i64, v_strides: *const i64, batch: i64, n_kv: c_int,
+        rows: i64, head_dim: c_int, max_seq: i64, pos: i64, positions: *const i32, lens: *const i32,
+        stream: *mut c_void) -> c_int;
+    pub fn rt_rope_kv4_append(q: *mut c_void, k_in: *const c_void, v_in: *const c_void, k_codes: *mut c_void,
+        k_scales: *mut c_void, v_codes: *mut c_void, v_scales: *mut c_void, inv_freq: *const f32, batch: i64,
+        n_heads: c_int, n_kv: c_int, head_dim: c_int, max_seq: i64, pos: i64, positions: *const i32, slot: i64,
+        slots: *const i32, rope_style: c_int, stream: *mut c_void) -> c_int;
+    pub fn rt_kv4_read(k_codes: *const c_void, k_scales: *const c_void, v_codes: *const c_void,
+        v_scales: *const c_void, k_out: *mut c_void, v_out: *mut c_void, batch: i64, n_kv: c_int, head_dim: c_int,
+        max_seq: i64, rows: i64, start: i64, starts: *const i32, kv_lens: *const i32, stream: *mut c_void) -> c_int;
+    pub fn rt_kv4_decode_workspace_bytes(batch: i64, n_heads: i64, n_kv_heads: i64, head_dim: c_int, max_seq: i64,
+        weighed: c_int) -> usize;
+    pub fn rt_kv4_decode(q: *const c_void, k_codes: *const c_void, k_scales: *const c_void, v_codes: *const c_void,
+        v_scales: *const c_void, out: *mut c_void, lse: *mut f32, weights: *mut f32, batch: i64, n_heads: i64,
+        n_kv_heads: i64, head_dim: c_int, max_seq: i64, kv_lens: *const i32, kv_len_uniform: i64, scale: f32,
+        workspace: *mut c_void, workspace_bytes: usize, stream: *mut c_void) -> c_int;
+    pub fn rt_kv_weigh_bf16(q: *const c_void, k_cache: *const c_void, lse: *const f32, weights: *mut f32, batch: i64,
+        n_heads: i64, n_kv_heads: i64, seq_q: i64, head_dim: c_int, max_seq: i64, kv_lens: *const i32,
+        kv_len_uniform: i64, scale: f32, stream: *mut c_void) -> c_int;
+    pub fn rt_kv_evict(src: *const *const c_void, dst: *const *mut c_void, row_bytes: *const i32, n_planes: c_int,
+        weights: *const f32, weights_out: *mut f32, kept: *mut i32, lens_out: *mut i32, batch: i64, n_kv_heads: i64,
+        max_seq: i64, max_seq_out: i64, kv_lens: *const i32, kv_len_uniform: i64, keep: i64, recent: i64,
+        stream: *mut c_void) -> c_int;
     pub fn rt_convert_f32_to_bf16(src: *const f32, dst: *mut c_void, n: i64, stream: *mut c_void) -> c_int;
     pub fn rt_convert_bf16_to_f32(src: *const c_void, dst: *mut f32, n: i64, stream: *mut c_void) -> c_int;
     pub fn rt_debug_tc_selftest(a: *const c_void, b: *const c_void, v: *const c_void, s_out: *mut f32,

@@ -106,6 +106,19 @@ PROTOTYPES = {
                                   c_void_p, c_void_p]),
     "rt_rope_kv_append_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int,
                                        c_int, c_int64, c_int64, c_void_p, c_int, c_void_p]),
+    "rt_kv4_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                              c_int, c_int64, c_int, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "rt_rope_kv4_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                   c_int, c_int, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p]),
+    "rt_kv4_read": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_int, c_int64,
+                            c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "rt_kv4_decode_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int64, c_int]),
+    "rt_kv4_decode": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                              c_int64, c_int64, c_int, c_int64, c_void_p, c_int64, c_float, c_void_p, c_size_t, c_void_p]),
+    "rt_kv_weigh_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_int, c_int64,
+                                 c_void_p, c_int64, c_float, c_void_p]),
+    "rt_kv_evict": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                            c_int64, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p]),
     "rt_convert_f32_to_bf16": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "rt_convert_bf16_to_f32": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "rt_debug_tc_selftest": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p]),
@@ -146,6 +159,17 @@ def torch_binding():
                                "`python -m rustorch_b200.build`") from e
         _binding = _torch_binding
     return _binding
+
+
+def _array(kind):
+    """Values -> a ctypes array of them, as the entries take their host arrays."""
+    def make(values):
+        values = list(values)
+        return (kind * len(values))(*values)
+    return make
+
+
+int64s, int32s, pointers = _array(c_int64), _array(c_int32), _array(c_void_p)
 
 
 def error_string(status: int) -> str:

@@ -1,0 +1,76 @@
+// Launch interface between the C ABI of the 4-bit cache and of eviction (api_cache.cu) and their kernels.
+#pragma once
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <type_traits>
+
+namespace rt {
+
+struct Kv4Cache {
+    const void *k_codes, *k_scales, *v_codes, *v_scales;  // written by the appends
+};
+
+template <class F>
+inline cudaError_t for_head_dim(int head_dim, F&& f) {
+    switch (head_dim) {
+        case 64: return f(std::integral_constant<int, 64>{});
+        case 128: return f(std::integral_constant<int, 128>{});
+        default: return f(std::integral_constant<int, 256>{});
+    }
+}
+
+// Launch with programmatic stream serialisation: the kernel may be resident before the one ahead of it in the stream has
+// ended, and waits for it on the device (griddepcontrol.wait) before it touches global memory.
+template <class... Params, class... Args>
+inline cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                                  const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// ---- kv4_rows.cu
+cudaError_t launch_kv4_append(const Kv4Cache& c, const void* k, const void* v, const int64_t* ks, const int64_t* vs,
+                              int64_t batch, int n_kv, int64_t rows, int head_dim, int64_t max_seq, int64_t pos,
+                              const int32_t* positions, const int32_t* lens, cudaStream_t stream);
+cudaError_t launch_rope_kv4_append(const Kv4Cache& c, void* q, const void* k, const void* v, const float* inv_freq,
+                                   int64_t batch, int n_heads, int n_kv, int head_dim, int64_t max_seq, int64_t pos,
+                                   const int32_t* positions, int64_t slot, const int32_t* slots, int style,
+                                   cudaStream_t stream);
+cudaError_t launch_kv4_read(const Kv4Cache& c, void* k, void* v, int64_t batch, int n_kv, int head_dim, int64_t max_seq,
+                            int64_t rows, int64_t start, const int32_t* starts, const int32_t* kv_lens, cudaStream_t stream);
+
+// ---- kv4_decode.cu
+size_t kv4_decode_workspace_bytes(int64_t batch, int n_heads, int n_kv, int head_dim, int64_t max_seq, bool weighed);
+cudaError_t launch_kv4_decode(const Kv4Cache& c, const void* q, void* out, float* lse, float* weights, int64_t batch,
+                              int n_heads, int n_kv, int head_dim, int64_t max_seq, const int32_t* kv_lens,
+                              int64_t kv_len_uniform, float scale, void* workspace, cudaStream_t stream);
+
+// ---- kv_weigh.cu
+cudaError_t launch_kv_weigh(const void* q, const void* k_cache, const float* lse, float* weights, int64_t batch, int n_heads,
+                            int n_kv, int64_t seq_q, int head_dim, int64_t max_seq, const int32_t* kv_lens,
+                            int64_t kv_len_uniform, float scale, cudaStream_t stream);
+
+// ---- kv_evict.cu
+struct EvictPlanes {
+    static constexpr int kMost = 4;
+    const void* src[kMost];
+    void* dst[kMost];
+    int row_bytes[kMost];
+    int n;
+};
+cudaError_t launch_kv_evict(const EvictPlanes& planes, const float* weights, float* weights_out, int32_t* kept,
+                            int32_t* lens_out, int64_t batch, int n_kv, int64_t max_seq, int64_t max_seq_out,
+                            const int32_t* kv_lens, int64_t kv_len_uniform, int64_t keep, int64_t recent,
+                            cudaStream_t stream);
+
+}  // namespace rt
