@@ -1,8 +1,12 @@
 // Single-token GQA attention over a 4-bit KV cache.
 //
-// out = sum_t p_t v_t, p = softmax(scale * q . k_t), with k, v = lo + scale * code per group of 32 values.  A CTA takes an
-// equal part of one (sequence, KV head)'s tokens in tiles of 64 with the running maximum and sum of a softmax; the G query
-// heads share every row that is read.  The parts' results are merged by their log-sum-exp.
+// out = sum_t p_t v_t, p = softmax(scale * q . k_t), with k, v = lo + scale * code per group of 32 values.  Per group
+//     q . k = scale * sum(q * code) + lo * sum(q),        sum_t p_t v_t = sum_t (p_t scale_t) code_t + sum_t p_t lo_t,
+// so the matrix instructions run on the bare codes and nothing is dequantised.  A code in the low bits of a 16-bit half is
+// the f16 subnormal code * 2^-24, which mma.sync multiplies exactly: one AND makes a pair of operands, and the high
+// nibble of a byte, 16 times as large, is met by a q (or a result row) that is 16 times as small.
+#include <algorithm>
+
 #include "cache_kernels.h"
 #include "kernels.h"
 #include "kv4.cuh"
@@ -10,163 +14,575 @@
 namespace rt {
 namespace {
 
-constexpr int kTile = 64, kThreads = 128, kMaxGroup = 8;
+constexpr int kWarps = 4, kThreads = 32 * kWarps, kMaxGroup = 8;
+constexpr int kStep = 32;    // tokens of a warp's step
+constexpr int kTile = 64;    // tokens of a unit of work: the tiles of a launch are dealt to the CTAs in equal runs
+constexpr float kLazy = 4.f; // log2 of what a probability may exceed 1 by before the running maximum moves
+
+template <int D>
+struct Shape {
+    using R = Kv4Row<D>;
+    static constexpr int kGroups = R::kGroups, kSpanGroups = R::kSpanGroups, kSpans = D / R::kSpan;
+    static constexpr int kRow = D / 2, kScaleRow = D / 8;
+    // Four lanes read rows 0, 2, 4 and 6 of V at a time: a pitch of 16 bytes more keeps them in different banks.
+    static constexpr int kVPitch = kRow + 16;
+    static constexpr int kKBytes = kStep * kRow, kVBytes = kStep * kVPitch, kScaleBytes = kStep * kScaleRow;
+    static constexpr int kStage = kKBytes + kVBytes + 2 * kScaleBytes;
+    static constexpr int kStages = D == 256 ? 2 : 3;  // steps of a warp in shared memory
+    static constexpr int kPerSm = D == 256 ? 2 : 3;   // CTAs resident on an SM
+    static constexpr int kSmem = kWarps * kStages * kStage;
+    // The warps' results lie over the ring once it has run dry.
+    static constexpr int kMerge = kWarps * (kMaxGroup * (D + kGroups) + 2 * kMaxGroup) * 4;
+    static_assert(kMerge <= kSmem && kStage % 16 == 0, "the merge fits the ring");
+};
 
 struct DecodeParams {
     const __nv_bfloat16* q;
-    const uint8_t *k_codes, *v_codes;
-    const uint32_t *k_scales, *v_scales;
+    const uint8_t *k_codes, *k_scales, *v_codes, *v_scales;
     __nv_bfloat16* out;
-    float *lse, *part_o, *part_lse, *weights;
-    int64_t max_seq, rows;
+    float* lse;
+    float* weights;
+    float* scores;   // [B * Hkv, max_seq, group] scaled scores (log2), where weights are asked for
+    float* part_o;   // [2 * CTAs][group][D]
+    float2* part_ml; // [2 * CTAs][group]: the reference that the part's sums are relative to (log2), the sum of its weights
+    int64_t max_seq;
     const int32_t* kv_lens;
-    int kv_len, n_kv, group, parts;
+    int kv_len, batch, n_kv, group, ctas;
     float scale_log2;
 };
 
-__device__ __forceinline__ int visible(const int32_t* kv_lens, int uniform, int64_t max_seq, int64_t b) {
-    return max(0, (int)min(kv_lens ? (int64_t)kv_lens[b] : (int64_t)uniform, max_seq));
+__device__ __forceinline__ int visible(const DecodeParams& p, int b) {
+    return max(0, (int)min(p.kv_lens ? (int64_t)p.kv_lens[b] : (int64_t)p.kv_len, p.max_seq));
 }
+// A sequence without tokens has one tile too: somebody has to write its zeros.
+__device__ __forceinline__ int tiles_of(int len) { return max(1, (len + kTile - 1) / kTile); }
 
-template <int D>
-__device__ __forceinline__ float value_at(const uint8_t* codes, const uint32_t* scales, int64_t row, int d) {
-    using R = Kv4Row<D>;
-    const uint32_t c = codes[row * R::kCodeBytes + d / 2] >> (4 * (d & 1)) & 15u;
-    return kv4_value(kv4_scale(scales[row * R::kGroups + R::group_of_octet(d / 8)]), c);
-}
+// Tiles are numbered sequence by sequence, KV head by KV head; CTA i takes [i * all / ctas, (i + 1) * all / ctas),
+// with no more CTAs than tiles, so that every one has a part.
+__device__ __forceinline__ int64_t share_start(int64_t i, int64_t all, int ctas) { return i * all / ctas; }
+__device__ __forceinline__ int share_of(int64_t tile, int64_t all, int ctas) { return (int)(((tile + 1) * ctas - 1) / all); }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads) kv4_decode_kernel(const DecodeParams p) {
-    __shared__ float q[kMaxGroup][D], s[kMaxGroup][kTile], alpha[kMaxGroup], sum[kMaxGroup], top[kMaxGroup];
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int tid = threadIdx.x, h = blockIdx.y, G = p.group;
-    const int64_t b = blockIdx.z, bh = b * p.n_kv + h;
-    const int len = visible(p.kv_lens, p.kv_len, p.max_seq, b);
-    const int size = (len + p.parts - 1) / p.parts;
-    const int lo = min(len, (int)blockIdx.x * size), hi = min(len, lo + size);
-    for (int i = tid; i < G * D; i += kThreads) q[i / D][i % D] = __bfloat162float(p.q[bh * G * D + i]);
-    if (tid < kMaxGroup) sum[tid] = 0.f, top[tid] = -INFINITY;
-    constexpr int kPer = (D + kThreads - 1) / kThreads;
-    float acc[kPer][kMaxGroup] = {};
-    __syncthreads();
-    for (int t0 = lo; t0 < hi; t0 += kTile) {
-        const int n = min(kTile, hi - t0);
-        for (int i = tid; i < G * kTile; i += kThreads) {
-            const int g = i / kTile, t = i % kTile;
-            float x = -INFINITY;
-            if (t < n) {
-                x = 0.f;
-                for (int d = 0; d < D; ++d) x = fmaf(q[g][d], value_at<D>(p.k_codes, p.k_scales, bh * p.max_seq + t0 + t, d), x);
-                x *= p.scale_log2;
-            }
-            s[g][t] = x;
-        }
-        __syncthreads();
-        for (int g = tid / 32; g < G; g += kThreads / 32) {
-            const int lane = tid % 32;
-            const float a = s[g][lane], c = s[g][lane + 32], old = top[g];
-            float m = fmaxf(fmaxf(a, c), old);
-            for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
-            const float ref = m == -INFINITY ? 0.f : m;
-            const float pa = exp2f(a - ref), pc = exp2f(c - ref);
-            float l = pa + pc;
-            for (int off = 16; off; off >>= 1) l += __shfl_xor_sync(kFullMask, l, off);
-            s[g][lane] = pa, s[g][lane + 32] = pc;
-            if (lane == 0) {
-                const float f = old == -INFINITY ? 0.f : exp2f(old - ref);
-                alpha[g] = f, sum[g] = sum[g] * f + l, top[g] = m;
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int d = tid + j * kThreads;
-            if (d < D) {
-                for (int g = 0; g < kMaxGroup; ++g)
-                    if (g < G) acc[j][g] *= alpha[g];
-                for (int t = 0; t < n; ++t) {
-                    const float v = value_at<D>(p.v_codes, p.v_scales, bh * p.max_seq + t0 + t, d);
-                    for (int g = 0; g < kMaxGroup; ++g)
-                        if (g < G) acc[j][g] = fmaf(s[g][t], v, acc[j][g]);
-                }
-            }
-        }
-        __syncthreads();
+// Sum of the tiles of sequences [0, n) and of all, for all threads of the CTA.
+__device__ __forceinline__ void count_tiles(const DecodeParams& p, int n, int64_t& before, int64_t& all) {
+    if (!p.kv_lens) {
+        const int64_t t = tiles_of(visible(p, 0));
+        before = t * n * p.n_kv, all = t * p.batch * p.n_kv;
+        return;
+    }
+    __shared__ int64_t sums[kWarps][2];
+    int64_t x = 0, y = 0;
+    for (int b = threadIdx.x; b < p.batch; b += kThreads) {
+        const int t = tiles_of(visible(p, b));
+        x += b < n ? t : 0, y += t;
     }
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int d = tid + j * kThreads;
-        if (d < D)
-            for (int g = 0; g < kMaxGroup; ++g)
-                if (g < G) {
-                    const float o = hi > lo ? acc[j][g] / sum[g] : 0.f;
-                    if (p.part_o) p.part_o[((int64_t)blockIdx.x * p.rows + bh * G + g) * D + d] = o;
-                    else p.out[(bh * G + g) * D + d] = __float2bfloat16(o);
-                }
+    for (int off = 16; off; off >>= 1) {
+        x += __shfl_xor_sync(kFullMask, x, off);
+        y += __shfl_xor_sync(kFullMask, y, off);
     }
-    if (tid < G) {
-        const float l = hi > lo ? top[tid] * kLn2 + logf(sum[tid]) : -INFINITY;
-        if (p.part_o) p.part_lse[(int64_t)blockIdx.x * p.rows + bh * G + tid] = l;
-        else if (p.lse) p.lse[bh * G + tid] = l;
+    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32][0] = x, sums[threadIdx.x / 32][1] = y;
+    __syncthreads();
+    before = all = 0;
+    for (int w = 0; w < kWarps; ++w) before += sums[w][0], all += sums[w][1];
+    before *= p.n_kv, all *= p.n_kv;
+    __syncthreads();
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {  // 8x8 matrix of 16-bit values, a row's pair a lane
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+    const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float low_half(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w & 0xffffu))); }
+
+// Asynchronous copy of kBytes; `there` false writes zeros (and reads nothing).
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, bool there) {
+    const int n = there ? kBytes : 0;
+    if constexpr (kBytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
+}
+
+// kWords neighbouring words of shared memory.
+template <int kWords>
+__device__ __forceinline__ void load_words(uint32_t (&w)[kWords], const uint8_t* p) {
+    if constexpr (kWords == 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(p);
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        w[0] = x.x, w[1] = x.y;
     }
 }
 
-// weights[t] += sum over the group of exp(score - lse), a thread a token.
+// One (sequence, KV head)'s queries as the B operand of the score products: lane (g, j) = (lane / 4, lane % 4) holds query
+// g's octets of quarter j.  The queries are scaled by a power of two that brings their largest value to 2^14, where
+// bf16's 8 bits fit f16 exactly (values 2^-31 of the largest and smaller lose bits).
 template <int D>
-__global__ void __launch_bounds__(kThreads) kv4_weigh_kernel(const DecodeParams p) {
-    __shared__ float q[kMaxGroup][D], lse[kMaxGroup];
+struct Queries {
+    uint32_t even[Shape<D>::kGroups][2], odd[Shape<D>::kGroups][2];  // pairs (0,4), (2,6) and (1,5)/16, (3,7)/16 of an octet
+    uint32_t sums[Shape<D>::kSpans][2];  // a group's sum / 64 in three f16 parts (and 0): 33 bits
+    float factor[2];                     // scale_log2 * 2^24 / the power of two, of queries 2j and 2j + 1
+
+    __device__ __forceinline__ void load(const DecodeParams& p, int64_t bh, int lane) {
+        using S = Shape<D>;
+        const int g = lane / 4, j = lane % 4;
+        uint4 raw[S::kGroups];
+        float top = 0.f;
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < S::kGroups; ++i) {
+            const int octet = (i / S::kSpanGroups) * S::R::kSpanOctets + j * S::kSpanGroups + i % S::kSpanGroups;
+            raw[i] = make_uint4(0, 0, 0, 0);
+            if (g < p.group) raw[i] = *reinterpret_cast<const uint4*>(p.q + (bh * p.group + g) * D + 8 * octet);
+            const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = bf16x2_to_float2(u[k]);
+                top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                nan |= f.x != f.x || f.y != f.y;
+            }
+        }
+        top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(kFullMask, top, 2));
+        const int e = top > 0.f && top < INFINITY ? 14 - (((int)(__float_as_uint(top) >> 23) & 255) - 127) : 0;
+        // 2^e in two factors: e may be past f32's exponents
+        const float up0 = __uint_as_float((uint32_t)(127 + e / 2) << 23), up1 = __uint_as_float((uint32_t)(127 + e - e / 2) << 23);
+        float total[S::kGroups];
+#pragma unroll
+        for (int i = 0; i < S::kGroups; ++i) {
+            const uint32_t u[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            float x[8];
+            total[i] = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = bf16x2_to_float2(u[k]);
+                x[2 * k] = f.x * up0 * up1, x[2 * k + 1] = f.y * up0 * up1;
+                total[i] += x[2 * k] + x[2 * k + 1];
+            }
+            total[i] += __shfl_xor_sync(kFullMask, total[i], 1);
+            total[i] += __shfl_xor_sync(kFullMask, total[i], 2);
+            even[i][0] = pack_half2(x[0], x[4]), even[i][1] = pack_half2(x[2], x[6]);
+            odd[i][0] = pack_half2(x[1] * 0.0625f, x[5] * 0.0625f), odd[i][1] = pack_half2(x[3] * 0.0625f, x[7] * 0.0625f);
+        }
+#pragma unroll
+        for (int s = 0; s < S::kSpans; ++s) {
+            float t = 0.f;  // lane j's group of the span
+#pragma unroll
+            for (int i = 0; i < S::kSpanGroups; ++i) t = j == i ? total[s * S::kSpanGroups + i] * 0.015625f : t;
+            const float a = __half2float(__float2half_rn(t)), b = __half2float(__float2half_rn(t - a));
+            sums[s][0] = pack_half2(a, b), sums[s][1] = pack_half2(t - a - b, 0.f);
+        }
+        // NaN and infinite queries: the row is NaN whatever the codes are
+        float f = nan || top == INFINITY ? __uint_as_float(0x7fffffffu) : p.scale_log2 * exp2f((float)(24 - e));
+        nan = (__ballot_sync(kFullMask, nan) >> (lane & ~3)) & 15u;
+        if (nan) f = __uint_as_float(0x7fffffffu);
+        factor[0] = __shfl_sync(kFullMask, f, 8 * j);
+        factor[1] = __shfl_sync(kFullMask, f, 8 * j + 4);
+    }
+};
+
+// What a warp has summed so far.  Lane (g, j) holds queries 2j and 2j + 1.
+template <int D>
+struct Sums {
+    float o[Shape<D>::kGroups][2][4];  // [group][dims 0-1, 2-3 of a lane's four]: codes, {q 2j, 2j+1} x {even, odd dim}
+    float lo[4];                       // sum p * lo, row g = group g
+    float ref[2], top[2], l[2];        // p = 2^(score - ref); running maximum; sum of p (this lane's tokens)
+};
+
+// 32 tokens (valid of them) that lie in shared memory.
+template <int D>
+__device__ __forceinline__ void step(const uint8_t* stage, int valid, const Queries<D>& q, Sums<D>& a, float& base,
+                                     uint32_t& scale_limit, int lane, float* scores, int group) {
+    using S = Shape<D>;
+    const int g = lane / 4, j = lane % 4;
+    const uint8_t *kc = stage, *vc = stage + S::kKBytes, *ks = vc + S::kVBytes, *vs = ks + S::kScaleBytes;
+    float x[2][4];
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb) {
+        const int r0 = tb * 16 + g, r1 = r0 + 8;
+        float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < S::kSpans; ++s) {  // sum(q) * lo: lane j brings its group
+            const int at = (s * S::kSpanGroups + (j & (S::kSpanGroups - 1))) * 4;
+            const uint32_t a0 = __byte_perm(*reinterpret_cast<const uint32_t*>(ks + r0 * S::kScaleRow + at), 0, 0x3232),
+                           a1 = __byte_perm(*reinterpret_cast<const uint32_t*>(ks + r1 * S::kScaleRow + at), 0, 0x3232);
+            mma_f16(m, a0, a1, a0, a1, q.sums[s][0], q.sums[s][1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[tb][k] = m[k] * 3.814697265625e-06f;  // 64 * 2^-24
+#pragma unroll
+        for (int s = 0; s < S::kSpans; ++s) {
+            uint32_t w0[S::kSpanGroups], w1[S::kSpanGroups], s0[S::kSpanGroups], s1[S::kSpanGroups];
+            // at D = 256 odd rows have their spans swapped, so that two rows fill all banks
+            const int swap = S::kSpans == 2 ? (g & 1) : 0;
+            load_words(w0, kc + r0 * S::kRow + (s ^ swap) * 64 + j * 4 * S::kSpanGroups);
+            load_words(w1, kc + r1 * S::kRow + (s ^ swap) * 64 + j * 4 * S::kSpanGroups);
+            load_words(s0, ks + r0 * S::kScaleRow + s * 4 * S::kSpanGroups);
+            load_words(s1, ks + r1 * S::kScaleRow + s * 4 * S::kSpanGroups);
+#pragma unroll
+            for (int i = 0; i < S::kSpanGroups; ++i) {
+                const int gi = s * S::kSpanGroups + i;
+                float c[4] = {0.f, 0.f, 0.f, 0.f};
+                mma_f16(c, w0[i] & 0x000f000fu, w1[i] & 0x000f000fu, w0[i] & 0x00f000f0u, w1[i] & 0x00f000f0u, q.even[gi][0],
+                        q.odd[gi][0]);
+                const uint32_t h0 = w0[i] >> 8, h1 = w1[i] >> 8;
+                mma_f16(c, h0 & 0x000f000fu, h1 & 0x000f000fu, h0 & 0x00f000f0u, h1 & 0x00f000f0u, q.even[gi][1], q.odd[gi][1]);
+                const float f0 = low_half(s0[i]), f1 = low_half(s1[i]);
+                x[tb][0] = fmaf(f0, c[0], x[tb][0]), x[tb][1] = fmaf(f0, c[1], x[tb][1]);
+                x[tb][2] = fmaf(f1, c[2], x[tb][2]), x[tb][3] = fmaf(f1, c[3], x[tb][3]);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[tb][k] *= q.factor[k & 1];
+    }
+    if (valid < kStep) {
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (tb * 16 + g + 4 * (k & 2) >= valid) x[tb][k] = -INFINITY;
+    }
+    if (scores) {  // [token][query]
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int t = tb * 16 + g + 4 * (k & 2), h = 2 * j + (k & 1);
+                if (t < valid && h < group) scores[t * group + h] = x[tb][k];
+            }
+    }
+    // The largest scale of V's 32 tokens: p is held times 2^base so that p * scale stays within f16.
+    uint32_t big = 0;
+#pragma unroll
+    for (int i = 0; i < S::kGroups; i += S::kSpanGroups) {
+        uint32_t w[S::kSpanGroups];
+        load_words(w, vs + lane * S::kScaleRow + 4 * i);
+#pragma unroll
+        for (int k = 0; k < S::kSpanGroups; ++k) big = max(big, w[k] & 0xffffu);
+    }
+    float top[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        float m = fmaxf(fmaxf(x[0][c], x[0][c + 2]), fmaxf(x[1][c], x[1][c + 2]));
+        m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 4));
+        m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 8));
+        top[c] = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16));
+    }
+    if (__any_sync(kFullMask, top[0] > a.top[0] + kLazy || top[1] > a.top[1] + kLazy || big > scale_limit)) {
+        big = __reduce_max_sync(kFullMask, big);
+        if (big > scale_limit) {  // s < 2^(exponent + 1)
+            scale_limit = big | 0x3ffu;
+            base = 15.f - kLazy - (float)((int)(big >> 10) - 14);
+        }
+        float alpha[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const bool first = a.top[c] == -INFINITY;
+            a.top[c] = fmaxf(a.top[c], top[c]);
+            const float ref = a.top[c] == -INFINITY ? 0.f : a.top[c] - base;
+            alpha[c] = first ? 1.f : exp2f(a.ref[c] - ref);
+            a.ref[c] = ref;
+            a.l[c] *= alpha[c];
+        }
+#pragma unroll
+        for (int i = 0; i < S::kGroups; ++i)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) a.o[i][t][k] *= alpha[k & 1];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a.lo[k] *= alpha[k & 1];
+    }
+    uint32_t prob[2][2];  // query g, tokens 2j, 2j + 1 (and 8 more) of a block of 16
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb) {
+        float e[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            e[k] = fast_exp2(x[tb][k] - a.ref[k & 1]);
+            a.l[k & 1] += e[k];
+        }
+        // rounded to f16's 11 bits (once more with the token's scale), 2^-4 of the result's own rounding to bf16
+        prob[tb][0] = transposed(pack_half2(e[0], e[1]));
+        prob[tb][1] = transposed(pack_half2(e[2], e[3]));
+    }
+    const uint32_t half_of = (g & 1) ? 0x7632u : 0x5410u;
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb) {
+        const int t = tb * 16 + 2 * j;
+        {  // sum p * lo: row g of the product is group g
+            const uint8_t* at = vs + t * S::kScaleRow + (g & (S::kGroups - 1)) * 4;
+            const uint32_t a0 = __byte_perm(*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + S::kScaleRow), 0x7632),
+                           a2 = __byte_perm(*reinterpret_cast<const uint32_t*>(at + 8 * S::kScaleRow),
+                                            *reinterpret_cast<const uint32_t*>(at + 9 * S::kScaleRow), 0x7632);
+            mma_f16(a.lo, a0, 0u, a2, 0u, prob[tb][0], prob[tb][1]);
+        }
+#pragma unroll
+        for (int s = 0; s < S::kSpans; ++s) {
+            uint32_t w[4][S::kSpanGroups], f[4][S::kSpanGroups];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int row = t + (k & 1) + 4 * (k & 2);
+                load_words(w[k], vc + row * S::kVPitch + s * 64 + (g >> 1) * 4 * S::kSpanGroups);
+                load_words(f[k], vs + row * S::kScaleRow + s * 4 * S::kSpanGroups);
+            }
+#pragma unroll
+            for (int i = 0; i < S::kSpanGroups; ++i) {
+                const int gi = s * S::kSpanGroups + i;
+                const uint32_t b0 = mul_half2(prob[tb][0], __byte_perm(f[0][i], f[1][i], 0x5410)),
+                               b1 = mul_half2(prob[tb][1], __byte_perm(f[2][i], f[3][i], 0x5410));
+                uint32_t p0 = __byte_perm(w[0][i], w[1][i], half_of), p1 = __byte_perm(w[2][i], w[3][i], half_of);
+                mma_f16(a.o[gi][0], p0 & 0x000f000fu, p0 & 0x00f000f0u, p1 & 0x000f000fu, p1 & 0x00f000f0u, b0, b1);
+                p0 >>= 8, p1 >>= 8;
+                mma_f16(a.o[gi][1], p0 & 0x000f000fu, p0 & 0x00f000f0u, p1 & 0x000f000fu, p1 & 0x00f000f0u, b0, b1);
+            }
+        }
+    }
+}
+
+// A warp's copies of 32 tokens from `from` on, `valid` of them, into a stage.
+template <int D>
+__device__ __forceinline__ void fetch(uint8_t* stage, const DecodeParams& p, int64_t row, int valid, int lane) {
+    using S = Shape<D>;
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(stage);
+    constexpr int kChunks = S::kRow / 16;  // of a row's codes
+#pragma unroll
+    for (int n = 0; n < kChunks; ++n) {
+        const int x = lane + 32 * n, r = x / kChunks, c = x % kChunks;
+        const bool there = r < valid;
+        const int64_t from = (row + (there ? r : 0)) * S::kRow + c * 16;
+        const int swapped = S::kSpans == 2 ? c ^ ((r & 1) << 2) : c;
+        copy_async<16>(to + r * S::kRow + swapped * 16, p.k_codes + from, there);
+        copy_async<16>(to + S::kKBytes + r * S::kVPitch + c * 16, p.v_codes + from, there);
+    }
+    constexpr int kPiece = S::kScaleRow < 16 ? S::kScaleRow : 16, kPieces = S::kScaleRow / kPiece;
+#pragma unroll
+    for (int n = 0; n < kPieces; ++n) {
+        const int x = lane + 32 * n, r = x / kPieces, c = x % kPieces;
+        const bool there = r < valid;
+        const int64_t from = (row + (there ? r : 0)) * S::kScaleRow + c * kPiece;
+        const uint32_t at = to + S::kKBytes + S::kVBytes + r * S::kScaleRow + c * kPiece;
+        copy_async<kPiece>(at, p.k_scales + from, there);
+        copy_async<kPiece>(at + S::kScaleBytes, p.v_scales + from, there);
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(const DecodeParams p) {
+    using S = Shape<D>;
+    constexpr int kStages = S::kStages;
+    extern __shared__ __align__(16) uint8_t smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int tid = threadIdx.x, h = blockIdx.y, G = p.group;
-    const int64_t b = blockIdx.z, bh = b * p.n_kv + h;
-    const int len = visible(p.kv_lens, p.kv_len, p.max_seq, b);
-    for (int i = tid; i < G * D; i += kThreads) q[i / D][i % D] = __bfloat162float(p.q[bh * G * D + i]);
-    if (tid < G) lse[tid] = p.lse[bh * G + tid] * kLog2e;
-    __syncthreads();
-    const int t = blockIdx.x * kThreads + tid;
-    if (t >= len) return;
-    float x[kMaxGroup] = {}, w = 0.f;
-    for (int d = 0; d < D; ++d) {
-        const float k = value_at<D>(p.k_codes, p.k_scales, bh * p.max_seq + t, d);
-        for (int g = 0; g < kMaxGroup; ++g)
-            if (g < G) x[g] = fmaf(q[g][d], k, x[g]);
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, G = p.group;
+    int64_t before, all;
+    count_tiles(p, 0, before, all);
+    const int ctas = (int)min((int64_t)p.ctas, all);
+    if (blockIdx.x >= ctas) return;
+    int64_t at = share_start(blockIdx.x, all, ctas);
+    const int64_t end = share_start(blockIdx.x + 1, all, ctas);
+    // the sequence of the first tile
+    int b = 0;
+    int64_t first = 0;  // its first tile
+    if (!p.kv_lens) {
+        const int64_t n = (int64_t)tiles_of(visible(p, 0)) * p.n_kv;
+        b = (int)(at / n), first = b * n;
+    } else {
+        for (int b0 = 0;; b0 += 32) {  // every warp on its own
+            const int64_t n = b0 + lane < p.batch ? (int64_t)tiles_of(visible(p, b0 + lane)) * p.n_kv : 0;
+            int64_t upto = n;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int64_t y = __shfl_up_sync(kFullMask, upto, off);
+                if (lane >= off) upto += y;
+            }
+            const unsigned owner = __ballot_sync(kFullMask, first + upto > at);
+            if (owner || b0 + 32 >= p.batch) {
+                const int o = owner ? __ffs(owner) - 1 : 31;
+                b = b0 + o, first += __shfl_sync(kFullMask, upto - n, o);
+                break;
+            }
+            first += __shfl_sync(kFullMask, upto, 31);
+        }
     }
-    for (int g = 0; g < kMaxGroup; ++g)
-        if (g < G) w += exp2f(x[g] * p.scale_log2 - lse[g]);
-    p.weights[bh * p.max_seq + t] += w;
+    uint8_t* ring = smem + warp * kStages * S::kStage;
+    for (bool head = true; at < end; head = false) {
+        const int len = visible(p, b), n = tiles_of(len);
+        const int h = (int)((at - first) / n), tile = (int)((at - first) % n);
+        const int tiles = (int)min(end - at, (int64_t)(n - tile));
+        const int lo = tile * kTile, hi = min(len, lo + tiles * kTile);
+        const int64_t bh = (int64_t)b * p.n_kv + h, rows = bh * p.max_seq;
+        const bool whole = tiles == n;
+        const int steps = (hi - lo + kStep - 1) / kStep;  // of the CTA; 0 without tokens
+        auto prefetch = [&](int s, int slot) {
+            if (s < steps) fetch<D>(ring + slot * S::kStage, p, rows + lo + s * kStep, min(kStep, hi - lo - s * kStep), lane);
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) prefetch(warp + i * kWarps, i);
+        Queries<D> q;
+        q.load(p, bh, lane);
+        Sums<D> a = {};
+        a.top[0] = a.top[1] = -INFINITY;
+        float base = 15.f - kLazy;
+        uint32_t scale_limit = 0x3bffu;  // scales below 1
+        int slot = 0;
+        for (int s = warp; s < steps; s += kWarps) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+            __syncwarp();
+            int next = slot + kStages - 1;
+            if (next >= kStages) next -= kStages;
+            prefetch(s + (kStages - 1) * kWarps, next);
+            const int t0 = lo + s * kStep;
+            step<D>(ring + slot * S::kStage, hi - t0, q, a, base, scale_limit, lane,
+                    p.scores ? p.scores + (rows + t0) * G : nullptr, G);
+            if (++slot == kStages) slot = 0;
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        // ---- the four warps' results, over the ring
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) a.l[c] += __shfl_xor_sync(kFullMask, a.l[c], off);
+        float* results = reinterpret_cast<float*>(smem);             // [warp][query][D + groups]
+        float2* ml = reinterpret_cast<float2*>(results + kWarps * kMaxGroup * (D + S::kGroups));  // [warp][query]
+        __syncthreads();
+        if (lane < 4) {
+            ml[warp * kMaxGroup + 2 * lane] = make_float2(a.top[0] == -INFINITY && a.l[0] == 0.f ? -INFINITY : a.ref[0], a.l[0]);
+            ml[warp * kMaxGroup + 2 * lane + 1] = make_float2(a.top[1] == -INFINITY && a.l[1] == 0.f ? -INFINITY : a.ref[1], a.l[1]);
+        }
+        __syncthreads();
+        {
+            const int g = lane / 4, j = lane % 4;
+            float f[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float m = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * kMaxGroup + 2 * j + c].x);
+                const float mine = ml[warp * kMaxGroup + 2 * j + c].x;
+                f[c] = mine == -INFINITY ? 0.f : exp2f(mine - m);
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                float* row = results + (warp * kMaxGroup + 2 * j + c) * (D + S::kGroups);
+                const float even = f[c] * 16777216.f, odd = f[c] * 1048576.f;  // 2^24, and 2^20 for the high nibbles
+#pragma unroll
+                for (int i = 0; i < S::kGroups; ++i)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const int d = (i / S::kSpanGroups) * S::R::kSpan + (g >> 1) * (S::R::kSpan / 4) + 8 * (i % S::kSpanGroups) +
+                                      4 * (g & 1) + 2 * t;
+                        row[d] = a.o[i][t][c] * even;
+                        row[d + 1] = a.o[i][t][c + 2] * odd;
+                    }
+                if (g < S::kGroups) row[D + g] = a.lo[c] * f[c];
+            }
+        }
+        __syncthreads();
+        const int64_t part = 2 * (int64_t)blockIdx.x + !head;
+        for (int i = tid; i < G * D; i += kThreads) {
+            const int h = i / D, d = i % D;
+            float m = -INFINITY, l = 0.f, o = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * kMaxGroup + h].x);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float2 x = ml[w * kMaxGroup + h];
+                const float* row = results + (w * kMaxGroup + h) * (D + S::kGroups);
+                l += x.x == -INFINITY ? 0.f : x.y * exp2f(x.x - m);
+                o += row[d] + row[D + S::R::group_of_octet(d / 8)];
+            }
+            if (whole) {
+                p.out[(bh * G + h) * D + d] = __float2bfloat16(hi > lo ? o / l : 0.f);
+                if (d == 0 && p.lse) p.lse[bh * G + h] = hi > lo ? m * kLn2 + logf(l) : -INFINITY;
+            } else {
+                p.part_o[(part * G + h) * D + d] = o;
+                if (d == 0) p.part_ml[part * G + h] = make_float2(m, l);
+            }
+        }
+        __syncthreads();
+        at += tiles;
+        if (h == p.n_kv - 1 && tile + tiles == n) first += (int64_t)n * p.n_kv, ++b;
+    }
 }
 
-// One CTA a row: the parts' results weighed by their log-sum-exp.  A NaN part makes the row NaN.
+// The parts of (sequence, KV head) blockIdx.x that several CTAs worked on, query blockIdx.y.
 __global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const DecodeParams p, int dim) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t row = blockIdx.x;
-    float top = -INFINITY;
-    for (int r = 0; r < p.parts; ++r) top = fmaxf(top, p.part_lse[r * p.rows + row]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    float total = 0.f;
-    for (int r = 0; r < p.parts; ++r) total += expf(p.part_lse[r * p.rows + row] - ref);
+    const int bh = blockIdx.x, b = bh / p.n_kv, h = blockIdx.y, G = p.group;
+    int64_t before, all;
+    count_tiles(p, b, before, all);
+    const int n = tiles_of(visible(p, b));
+    const int64_t t0 = before + (int64_t)(bh % p.n_kv) * n;
+    const int ctas = (int)min((int64_t)p.ctas, all);
+    const int i0 = share_of(t0, all, ctas), i1 = share_of(t0 + n - 1, all, ctas);
+    if (i0 == i1) return;  // one CTA had all of it
+    // the first CTA's part is its last one, unless it begins with it
+    const int64_t head = 2 * (int64_t)i0 + (share_start(i0, all, ctas) < t0);
+    auto part = [&](int i) { return i == i0 ? head : 2 * (int64_t)i; };
+    float m = -INFINITY, l = 0.f;
+    for (int i = i0; i <= i1; ++i) m = fmaxf(m, p.part_ml[part(i) * G + h].x);
+    for (int i = i0; i <= i1; ++i) {
+        const float2 x = p.part_ml[part(i) * G + h];
+        l += x.y * exp2f(x.x - m);
+    }
+    const int64_t row = (int64_t)bh * G + h;
     for (int d = threadIdx.x; d < dim; d += kThreads) {
         float o = 0.f;
-        for (int r = 0; r < p.parts; ++r)
-            o += expf(p.part_lse[r * p.rows + row] - ref) * p.part_o[(r * p.rows + row) * dim + d];
-        p.out[row * dim + d] = __float2bfloat16(total == 0.f ? 0.f : o / total);
+        for (int i = i0; i <= i1; ++i) o = fmaf(p.part_o[(part(i) * G + h) * dim + d], exp2f(p.part_ml[part(i) * G + h].x - m), o);
+        p.out[row * dim + d] = __float2bfloat16(o / l);
     }
-    if (threadIdx.x == 0 && p.lse) p.lse[row] = ref + logf(total);
+    if (threadIdx.x == 0 && p.lse) p.lse[row] = m * kLn2 + logf(l);
 }
 
-int parts_of(int64_t batch, int n_kv, int64_t max_seq) {
-    const int64_t groups = batch * n_kv, want = (4 * (int64_t)sm_count() + groups - 1) / groups;
-    return (int)max((int64_t)1, min(want, (max_seq + kTile - 1) / kTile));
+// weights[t] += sum over the group of 2^(score - lse): a thread a token.
+__global__ void __launch_bounds__(kThreads) kv4_weights_kernel(const DecodeParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t b = blockIdx.z, bh = b * p.n_kv + blockIdx.y;
+    const int len = visible(p, (int)b), t = blockIdx.x * kThreads + threadIdx.x;
+    if (t >= len) return;
+    const float* x = p.scores + (bh * p.max_seq + t) * p.group;
+    float w = 0.f;
+    for (int h = 0; h < p.group; ++h) w += exp2f(x[h] - p.lse[bh * p.group + h] * kLog2e);
+    p.weights[bh * p.max_seq + t] += w;
 }
+
+// CTAs of a launch: as many as fit at a time, or one for every tile.
+int ctas_of(int64_t batch, int n_kv, int head_dim, int64_t max_seq) {
+    const int per_sm = head_dim == 64 ? Shape<64>::kPerSm : head_dim == 128 ? Shape<128>::kPerSm : Shape<256>::kPerSm;
+    const int64_t tiles = batch * n_kv * ((max_seq + kTile - 1) / kTile);
+    return (int)std::min(tiles, (int64_t)per_sm * sm_count());
+}
+
+inline size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 }  // namespace
 
 size_t kv4_decode_workspace_bytes(int64_t batch, int n_heads, int n_kv, int head_dim, int64_t max_seq, bool weighed) {
-    const int parts = parts_of(batch, n_kv, max_seq);
-    const size_t rows = (size_t)batch * n_heads;
-    return (parts > 1 ? (size_t)parts * rows * (head_dim + 1) * sizeof(float) : 0) + (weighed ? rows * sizeof(float) : 0);
+    const size_t rows = 2 * (size_t)ctas_of(batch, n_kv, head_dim, max_seq) * (n_heads / n_kv + (n_heads % n_kv != 0));
+    return round16(rows * head_dim * sizeof(float)) + round16(rows * sizeof(float2)) +
+           (weighed ? round16((size_t)batch * n_heads * sizeof(float)) + round16((size_t)batch * n_heads * max_seq * sizeof(float)) : 0);
 }
 
 cudaError_t launch_kv4_decode(const Kv4Cache& c, const void* q, void* out, float* lse, float* weights, int64_t batch,
@@ -175,25 +591,30 @@ cudaError_t launch_kv4_decode(const Kv4Cache& c, const void* q, void* out, float
     DecodeParams p = {};
     p.q = (const __nv_bfloat16*)q;
     p.k_codes = (const uint8_t*)c.k_codes, p.v_codes = (const uint8_t*)c.v_codes;
-    p.k_scales = (const uint32_t*)c.k_scales, p.v_scales = (const uint32_t*)c.v_scales;
+    p.k_scales = (const uint8_t*)c.k_scales, p.v_scales = (const uint8_t*)c.v_scales;
     p.out = (__nv_bfloat16*)out, p.weights = weights;
-    p.max_seq = max_seq, p.rows = batch * n_heads, p.kv_lens = kv_lens, p.kv_len = (int)kv_len_uniform;
-    p.n_kv = n_kv, p.group = n_heads / n_kv, p.parts = parts_of(batch, n_kv, max_seq);
+    p.max_seq = max_seq, p.kv_lens = kv_lens, p.kv_len = (int)kv_len_uniform, p.batch = (int)batch;
+    p.n_kv = n_kv, p.group = n_heads / n_kv, p.ctas = ctas_of(batch, n_kv, head_dim, max_seq);
     p.scale_log2 = scale * kLog2e;
-    float* ws = static_cast<float*>(workspace);
-    if (p.parts > 1) {
-        p.part_o = ws, p.part_lse = ws + (size_t)p.parts * p.rows * head_dim;
-        ws = p.part_lse + (size_t)p.parts * p.rows;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    const size_t rows = 2 * (size_t)p.ctas * p.group;
+    p.part_o = (float*)ws, ws += round16(rows * head_dim * sizeof(float));
+    p.part_ml = (float2*)ws, ws += round16(rows * sizeof(float2));
+    if (weights) {
+        if (!lse) lse = (float*)ws;
+        ws += round16((size_t)batch * n_heads * sizeof(float));
+        p.scores = (float*)ws;
     }
-    if (!lse && weights) lse = ws;
     p.lse = lse;
     return for_head_dim(head_dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
-        cudaError_t e = launch_chained(kv4_decode_kernel<D>, dim3(p.parts, n_kv, (unsigned)batch), kThreads, 0, stream, p);
-        if (e == cudaSuccess && p.parts > 1)
-            e = launch_chained(kv4_merge_kernel, dim3((unsigned)p.rows), kThreads, 0, stream, p, D);
+        cudaError_t e = set_max_dynamic_smem_once<kv4_decode_kernel<D>>(Shape<D>::kSmem);
+        if (e != cudaSuccess) return e;
+        e = launch_chained(kv4_decode_kernel<D>, dim3(p.ctas), kThreads, Shape<D>::kSmem, stream, p);
+        if (e == cudaSuccess && p.ctas > 1)
+            e = launch_chained(kv4_merge_kernel, dim3((unsigned)(batch * n_kv), p.group), kThreads, 0, stream, p, D);
         if (e == cudaSuccess && weights)
-            e = launch_chained(kv4_weigh_kernel<D>, dim3((unsigned)((max_seq + kThreads - 1) / kThreads), n_kv, (unsigned)batch),
+            e = launch_chained(kv4_weights_kernel, dim3((unsigned)((max_seq + kThreads - 1) / kThreads), n_kv, (unsigned)batch),
                                kThreads, 0, stream, p);
         return e;
     });
