@@ -1,13 +1,21 @@
 // Softmax weights of queries over a bf16 cache, summed into an accumulator:
-//   weights[t] += sum over the queries i and heads g that share K of exp2(scale_log2 * q . k_t - lse_log2),  t <= len - seq_q + i.
+//   weights[t] += sum over the queries i and heads g that share K of 2^(scale_log2 * q . k_t - lse_log2),  t <= len - seq_q + i.
+//
+// A warp owns 16 or 32 tokens: their keys are the A operand of mma.sync.m16n8k16 and stay in registers (each lane loads 16
+// neighbouring values of a row, which are the k pairs of two products: the order of k is free as long as q has the same),
+// while the query rows pass by as B operands, eight at a time.  Every weight has one writer and is touched once.
+//
+// What bounds it: with one query a sequence, the keys' bytes; with a prompt's last queries, the exponentials and products.
 #include "cache_kernels.h"
 #include "kernels.h"
 #include "common.cuh"
+#include "mma_sync.cuh"
 
 namespace rt {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kBlock = 64;  // query rows in shared memory at a time
 
 struct WeighParams {
     const __nv_bfloat16 *q, *k;
@@ -19,31 +27,124 @@ struct WeighParams {
     float scale_log2;
 };
 
-// A thread a token; the query rows pass through shared memory one at a time.
 template <int D>
+struct WeighShape {
+    static constexpr int kTiles = D == 256 ? 1 : 2;  // of 16 tokens a warp: their keys take D / 4 registers a lane each
+    static constexpr int kTokens = 16 * kTiles * kWarps;
+    static constexpr int kChunks = D / 32;           // 16-byte pieces of a row per lane
+    static constexpr int kPitch = 2 * D + 64;        // of a query row in shared memory: two rows fill all banks
+};
+
+__device__ __forceinline__ float lse_log2(float lse) {  // a row that saw nothing adds nothing
+    return lse == -INFINITY ? INFINITY : lse * kLog2e;
+}
+
+// Scores of 16 tokens and 8 query rows, as accumulators of (row t = g or g + 8, queries 2j and 2j + 1).
+template <int D>
+__device__ __forceinline__ void scores(float (&c)[4], const uint4 (&k)[WeighShape<D>::kChunks][2], const uint4 (&q)[WeighShape<D>::kChunks]) {
+    c[0] = c[1] = c[2] = c[3] = 0.f;
+#pragma unroll
+    for (int n = 0; n < WeighShape<D>::kChunks; ++n) {
+        const uint32_t a[4] = {k[n][0].x, k[n][1].x, k[n][0].y, k[n][1].y}, b[4] = {k[n][0].z, k[n][1].z, k[n][0].w, k[n][1].w};
+        mma_bf16(c, a, q[n].x, q[n].y);
+        mma_bf16(c, b, q[n].z, q[n].w);
+    }
+}
+
+// kSingle: one query a sequence, its rows in registers.
+template <int D, bool kSingle>
 __global__ void __launch_bounds__(kThreads) kv_weigh_kernel(const WeighParams p) {
-    __shared__ float q[D];
+    using S = WeighShape<D>;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int h = blockIdx.y;
-    const int64_t b = blockIdx.z, bh = b * p.n_kv + h;
-    const int64_t len = max((int64_t)0, min(p.kv_lens ? (int64_t)p.kv_lens[b] : (int64_t)p.kv_len, p.max_seq));
-    const int64_t t = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-    const __nv_bfloat16* k = p.k + (bh * p.max_seq + min(t, p.max_seq - 1)) * D;
-    float w = 0.f;
-    for (int64_t r = 0; r < p.group * p.seq_q; ++r) {
-        const int64_t row = bh * p.group * p.seq_q + r;
-        __syncthreads();
-        for (int d = threadIdx.x; d < D; d += kThreads) q[d] = __bfloat162float(p.q[row * D + d]);
-        __syncthreads();
-        const float lse = p.lse[row];
-        if (t < len && t <= len - p.seq_q + r % p.seq_q && lse != -INFINITY) {
-            float x = 0.f;
-            for (int d = 0; d < D; ++d) x = fmaf(q[d], __bfloat162float(k[d]), x);
-            w += exp2f(x * p.scale_log2 - lse * kLog2e);
+    const int tid = threadIdx.x, lane = tid % 32, g = lane / 4, j = lane % 4;
+    const int64_t b = blockIdx.z, bh = b * p.n_kv + blockIdx.y;
+    const int len = max(0, (int)min(p.kv_lens ? (int64_t)p.kv_lens[b] : (int64_t)p.kv_len, p.max_seq));
+    const int first = blockIdx.x * S::kTokens;
+    if (first >= len) return;
+    const int t0 = first + (tid / 32) * 16 * S::kTiles;
+    uint4 k[S::kTiles][S::kChunks][2];
+#pragma unroll
+    for (int m = 0; m < S::kTiles; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            const int t = t0 + 16 * m + 8 * r + g;
+            const __nv_bfloat16* row = p.k + (bh * p.max_seq + min(t, len - 1)) * D + 8 * j;
+#pragma unroll
+            for (int n = 0; n < S::kChunks; ++n) k[m][n][r] = ld_stream_16B(row + 32 * n);
+        }
+    float w[S::kTiles][2] = {};
+    const int64_t row0 = bh * p.group * p.seq_q;
+    if constexpr (kSingle) {
+        uint4 q[S::kChunks];
+#pragma unroll
+        for (int n = 0; n < S::kChunks; ++n) {
+            q[n] = make_uint4(0, 0, 0, 0);
+            if (g < p.group) q[n] = *reinterpret_cast<const uint4*>(p.q + (row0 + g) * D + 32 * n + 8 * j);
+        }
+        float l[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) l[c] = 2 * j + c < p.group ? lse_log2(p.lse[row0 + 2 * j + c]) : INFINITY;
+#pragma unroll
+        for (int m = 0; m < S::kTiles; ++m) {
+            float c[4];
+            scores<D>(c, k[m], q);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[m][i / 2] += fast_exp2(fmaf(c[i], p.scale_log2, -l[i & 1]));
+        }
+    } else {
+        extern __shared__ __align__(16) uint8_t smem[];
+        __shared__ float s_lse[kBlock];
+        __shared__ int s_last[kBlock];  // the last token that a row sees
+        const int64_t rows = p.group * p.seq_q;
+        // the first query's place: whether any row of this warp's tokens can be hidden
+        const bool all_seen = t0 + 16 * S::kTiles - 1 <= len - p.seq_q;
+        for (int64_t r0 = 0; r0 < rows; r0 += kBlock) {
+            const int n_rows = (int)min((int64_t)kBlock, rows - r0);
+            __syncthreads();
+            for (int i = tid; i < kBlock * (D / 8); i += kThreads) {
+                const int r = i / (D / 8), c = i % (D / 8);
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (r < n_rows) x = *reinterpret_cast<const uint4*>(p.q + (row0 + r0 + r) * D + 8 * c);
+                *reinterpret_cast<uint4*>(smem + r * S::kPitch + 16 * c) = x;
+            }
+            if (tid < kBlock) {
+                const int64_t r = r0 + tid;
+                s_lse[tid] = tid < n_rows ? lse_log2(p.lse[row0 + r]) : INFINITY;
+                s_last[tid] = (int)(len - p.seq_q + r % p.seq_q);
+            }
+            __syncthreads();
+            if (t0 >= len) continue;
+            for (int n0 = 0; n0 < n_rows; n0 += 8) {
+                uint4 q[S::kChunks];
+#pragma unroll
+                for (int n = 0; n < S::kChunks; ++n)
+                    q[n] = *reinterpret_cast<const uint4*>(smem + (n0 + g) * S::kPitch + 64 * n + 16 * j);
+                const float2 l = *reinterpret_cast<const float2*>(&s_lse[n0 + 2 * j]);
+#pragma unroll
+                for (int m = 0; m < S::kTiles; ++m) {
+                    float c[4];
+                    scores<D>(c, k[m], q);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float e = fast_exp2(fmaf(c[i], p.scale_log2, i & 1 ? -l.y : -l.x));
+                        if (!all_seen && t0 + 16 * m + 4 * (i & 2) + g > s_last[n0 + 2 * j + (i & 1)]) e = 0.f;
+                        w[m][i / 2] += e;
+                    }
+                }
+            }
         }
     }
-    if (t < len) p.weights[bh * p.max_seq + t] += w;
+#pragma unroll
+    for (int m = 0; m < S::kTiles; ++m)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+            float x = w[m][r];
+            x += __shfl_xor_sync(kFullMask, x, 1);
+            x += __shfl_xor_sync(kFullMask, x, 2);
+            const int t = t0 + 16 * m + 8 * r + g;
+            if (j == 0 && t < len) p.weights[bh * p.max_seq + t] += x;
+        }
 }
 
 }  // namespace
@@ -55,9 +156,14 @@ cudaError_t launch_kv_weigh(const void* q, const void* k_cache, const float* lse
     p.q = (const __nv_bfloat16*)q, p.k = (const __nv_bfloat16*)k_cache, p.lse = lse, p.weights = weights;
     p.max_seq = max_seq, p.seq_q = seq_q, p.kv_lens = kv_lens, p.kv_len = (int)kv_len_uniform;
     p.n_kv = n_kv, p.group = n_heads / n_kv, p.scale_log2 = scale * kLog2e;
-    const dim3 grid((unsigned)((max_seq + kThreads - 1) / kThreads), n_kv, (unsigned)batch);
+    const int64_t longest = kv_lens ? max_seq : kv_len_uniform;
+    if (longest == 0) return cudaSuccess;
     return for_head_dim(head_dim, [&](auto d) {
-        return launch_chained(kv_weigh_kernel<decltype(d)::value>, grid, kThreads, 0, stream, p);
+        constexpr int D = decltype(d)::value;
+        using S = WeighShape<D>;
+        const dim3 grid((unsigned)((longest + S::kTokens - 1) / S::kTokens), n_kv, (unsigned)batch);
+        if (seq_q == 1) return launch_chained(kv_weigh_kernel<D, true>, grid, kThreads, 0, stream, p);
+        return launch_chained(kv_weigh_kernel<D, false>, grid, kThreads, (size_t)kBlock * S::kPitch, stream, p);
     });
 }
 
