@@ -15,6 +15,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -389,6 +390,258 @@ PyObject* backward(PyObject*, PyObject* const* arg, Py_ssize_t n) {
     });
 }
 
+// ---- a 4-bit cache and eviction.  These launch on the tensors' own device, whichever is current.
+
+// The planes of a Kv4Cache (a tuple; the wrapper has looked at its type).
+struct Kv4Args {
+    const Tensor* plane[4];
+    int64_t B, Hkv, S, D;
+    at::Device dev = at::Device(at::kCPU);
+};
+inline bool kv4_args(PyObject* o, Kv4Args& a) {
+    if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+    for (int i = 0; i < 4; ++i)
+        if (!(a.plane[i] = tensor_arg(PyTuple_GET_ITEM(o, i)))) return false;
+    const Tensor& c = *a.plane[0];
+    if (!c.is_cuda() || c.dim() != 4) return false;
+    a.dev = c.device();
+    a.B = c.size(0), a.Hkv = c.size(1), a.S = c.size(2), a.D = 2 * c.size(3);
+    for (int i = 0; i < 4; ++i) {
+        const Tensor& t = *a.plane[i];
+        if (!dense(t, i % 2 ? at::kHalf : at::kByte, a.dev) || t.size(0) != a.B || t.size(1) != a.Hkv || t.size(2) != a.S) return false;
+        if (i % 2 ? t.dim() != 5 || t.size(3) != a.D / 32 || t.size(4) != 2 : t.dim() != 4 || t.size(3) != a.D / 2) return false;
+    }
+    return true;
+}
+inline bool optional_vector(PyObject* o, const Tensor*& t, int64_t n, const at::Device& dev) {
+    return optional_arg(o, t) && (!t || (vector_of(*t, n, dev) && t->dim() == 1));
+}
+inline bool shaped(const Tensor& t, at::ScalarType type, const at::Device& dev, at::IntArrayRef sizes) {
+    return dense(t, type, dev) && t.sizes() == sizes;
+}
+inline void* stream_of(const at::Device& dev) { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+
+// cache, k, v, pos, positions, lens; True when done
+PyObject* kv4_append(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Kv4Args a;
+        if (n != 6 || !kv4_args(arg[0], a)) Py_RETURN_NONE;
+        const Tensor *x[2] = {tensor_arg(arg[1]), tensor_arg(arg[2])}, *positions, *lens;
+        int64_t pos, rows = -1, strides[2][3];
+        if (!x[0] || !x[1] || !int_arg(arg[3], pos, 0) || !optional_vector(arg[4], positions, a.B, a.dev) ||
+            !optional_vector(arg[5], lens, a.B, a.dev))
+            Py_RETURN_NONE;
+        for (int i = 0; i < 2; ++i) {
+            const Tensor& t = *x[i];
+            const int64_t d = t.dim(), T = d == 4 ? t.size(2) : 1;
+            if (!is(t, kBf16, a.dev) || (d != 3 && d != 4) || t.size(0) != a.B || t.size(1) != a.Hkv || t.size(d - 1) != a.D ||
+                (i && T != rows) || t.numel() == 0 || t.stride(d - 1) != 1)
+                Py_RETURN_NONE;
+            rows = T;
+            const int64_t size[3] = {a.B, a.Hkv, T}, step[3] = {t.stride(0), t.stride(1), d == 4 ? t.stride(2) : 0};
+            for (int k = 0; k < 3; ++k) strides[i][k] = size[k] == 1 ? 0 : step[k];
+        }
+        const c10::cuda::CUDAGuard guard(a.dev);
+        void* stream = stream_of(a.dev);
+        const int rc = unlocked([&] {
+            return rt_kv4_append(ptr(a.plane[0]), ptr(a.plane[1]), ptr(a.plane[2]), ptr(a.plane[3]), ptr(x[0]), ptr(x[1]), strides[0],
+                                 strides[1], a.B, (int)a.Hkv, rows, (int)a.D, a.S, pos, ptr<int32_t>(positions), ptr<int32_t>(lens), stream);
+        });
+        if (rc != RT_OK) Py_RETURN_NONE;
+        Py_RETURN_TRUE;
+    });
+}
+
+// q, k_in, v_in, cache, inv_freq, pos, positions, slot, slots, style (RT_ROPE_*); True when done
+PyObject* rope_kv4_append(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Kv4Args a;
+        if (n != 10 || !kv4_args(arg[3], a)) Py_RETURN_NONE;
+        const Tensor *q = tensor_arg(arg[0]), *k = tensor_arg(arg[1]), *v = tensor_arg(arg[2]), *freq = tensor_arg(arg[4]), *positions, *slots;
+        int64_t pos, slot, style;
+        if (!q || !k || !v || !freq || !int_arg(arg[5], pos, 0) || !optional_vector(arg[6], positions, a.B, a.dev) ||
+            !int_arg(arg[7], slot, -1) || !optional_vector(arg[8], slots, a.B, a.dev) || !int_arg(arg[9], style, -1))
+            Py_RETURN_NONE;
+        if (arg[7] != Py_None && slot < 0) Py_RETURN_NONE;
+        if (!dense(*q, kBf16, a.dev) || q->dim() != 3 || q->size(0) != a.B || q->size(2) != a.D ||
+            !shaped(*k, kBf16, a.dev, {a.B, a.Hkv, a.D}) || !shaped(*v, kBf16, a.dev, {a.B, a.Hkv, a.D}) ||
+            !shaped(*freq, kF32, a.dev, {a.D / 2}))
+            Py_RETURN_NONE;
+        const c10::cuda::CUDAGuard guard(a.dev);
+        void* stream = stream_of(a.dev);
+        const int rc = unlocked([&] {
+            return rt_rope_kv4_append(ptr(q), ptr(k), ptr(v), ptr(a.plane[0]), ptr(a.plane[1]), ptr(a.plane[2]), ptr(a.plane[3]),
+                                      ptr<float>(freq), a.B, (int)q->size(1), (int)a.Hkv, (int)a.D, a.S, pos, ptr<int32_t>(positions),
+                                      slot, ptr<int32_t>(slots), (int)style, stream);
+        });
+        if (rc != RT_OK) Py_RETURN_NONE;
+        Py_RETURN_TRUE;
+    });
+}
+
+// cache, rows, start, starts, kv_lens, out (None or a pair) -> (k, v)
+PyObject* kv4_read(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Kv4Args a;
+        if (n != 6 || !kv4_args(arg[0], a)) Py_RETURN_NONE;
+        const Tensor *starts, *lens, *out[2];
+        int64_t rows, start;
+        if (!int_arg(arg[1], rows, -1) || rows < 0 || !int_arg(arg[2], start, 0) || !optional_vector(arg[3], starts, a.B, a.dev) ||
+            !optional_vector(arg[4], lens, a.B, a.dev))
+            Py_RETURN_NONE;
+        Tensor fresh[2];
+        for (int i = 0; i < 2; ++i) {
+            if (arg[5] == Py_None) {
+                fresh[i] = empty({a.B, a.Hkv, rows, a.D}, kBf16, a.dev);
+                out[i] = &fresh[i];
+            } else {
+                if (!PyTuple_Check(arg[5]) || PyTuple_GET_SIZE(arg[5]) != 2 || !(out[i] = tensor_arg(PyTuple_GET_ITEM(arg[5], i))) ||
+                    !shaped(*out[i], kBf16, a.dev, {a.B, a.Hkv, rows, a.D}))
+                    Py_RETURN_NONE;
+            }
+        }
+        const c10::cuda::CUDAGuard guard(a.dev);
+        void* stream = stream_of(a.dev);
+        const int rc = unlocked([&] {
+            return rt_kv4_read(ptr(a.plane[0]), ptr(a.plane[1]), ptr(a.plane[2]), ptr(a.plane[3]), ptr(out[0]), ptr(out[1]), a.B,
+                               (int)a.Hkv, (int)a.D, a.S, rows, start, ptr<int32_t>(starts), ptr<int32_t>(lens), stream);
+        });
+        if (rc != RT_OK) Py_RETURN_NONE;
+        return pair(*out[0], out[1]);
+    });
+}
+
+// q, cache, kv_lens, kv_len, scale, return_lse, weights, workspace, out, lse -> (out, lse)
+PyObject* kv4_decode(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        Kv4Args a;
+        if (n != 10 || !kv4_args(arg[1], a)) Py_RETURN_NONE;
+        const Tensor *q = tensor_arg(arg[0]), *lens, *weights, *ws, *out, *lse;
+        int64_t kv_len;
+        float scale;
+        bool want_lse;
+        if (!q || !dense(*q, kBf16, a.dev) || q->dim() != 3 || q->size(0) != a.B || q->size(2) != a.D ||
+            !optional_vector(arg[2], lens, a.B, a.dev) || !int_arg(arg[3], kv_len, 0) || !scale_arg(arg[4], scale) ||
+            !flag_arg(arg[5], want_lse) || !optional_arg(arg[6], weights) || !optional_arg(arg[7], ws) || !optional_arg(arg[8], out) ||
+            !optional_arg(arg[9], lse))
+            Py_RETURN_NONE;
+        const int64_t Hq = q->size(1);
+        if ((weights && !shaped(*weights, kF32, a.dev, {a.B, a.Hkv, a.S})) || (ws && !dense(*ws, at::kByte, a.dev)) ||
+            (out && !shaped(*out, kBf16, a.dev, q->sizes())) || (lse && !shaped(*lse, kF32, a.dev, {a.B, Hq})))
+            Py_RETURN_NONE;
+        Tensor new_out, new_lse, new_ws;
+        if (!out) {
+            new_out = empty(q->sizes(), kBf16, a.dev);
+            out = &new_out;
+        }
+        if (!lse && want_lse) {
+            new_lse = empty({a.B, Hq}, kF32, a.dev);
+            lse = &new_lse;
+        }
+        const c10::cuda::CUDAGuard guard(a.dev);
+        if (!ws) {
+            const size_t need = rt_kv4_decode_workspace_bytes(a.B, Hq, a.Hkv, (int)a.D, a.S, weights != nullptr);
+            if (need) {
+                new_ws = empty({(int64_t)need}, at::kByte, a.dev);
+                ws = &new_ws;
+            }
+        }
+        void* stream = stream_of(a.dev);
+        const int rc = unlocked([&] {
+            return rt_kv4_decode(ptr(q), ptr(a.plane[0]), ptr(a.plane[1]), ptr(a.plane[2]), ptr(a.plane[3]), ptr(out), ptr<float>(lse),
+                                 ptr<float>(weights), a.B, Hq, a.Hkv, (int)a.D, a.S, ptr<int32_t>(lens), kv_len, scale, ptr(ws),
+                                 ws ? (size_t)ws->numel() : 0, stream);
+        });
+        if (rc != RT_OK) Py_RETURN_NONE;
+        return pair(*out, lse);
+    });
+}
+
+// q, k_cache, lse, weights, kv_lens, kv_len, scale; True when done
+PyObject* kv_weigh(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 7) Py_RETURN_NONE;
+        const Tensor *q = tensor_arg(arg[0]), *k = tensor_arg(arg[1]), *lse = tensor_arg(arg[2]), *w = tensor_arg(arg[3]), *lens;
+        int64_t kv_len;
+        float scale;
+        if (!q || !k || !lse || !w || !k->is_cuda() || k->dim() != 4 || (q->dim() != 3 && q->dim() != 4)) Py_RETURN_NONE;
+        const at::Device dev = k->device();
+        const int64_t B = k->size(0), Hkv = k->size(1), S = k->size(2), D = k->size(3), Hq = q->size(1), T = q->dim() == 4 ? q->size(2) : 1;
+        if (!dense(*k, kBf16, dev) || !dense(*q, kBf16, dev) || q->size(0) != B || q->size(-1) != D ||
+            !shaped(*lse, kF32, dev, q->sizes().slice(0, q->dim() - 1)) || !shaped(*w, kF32, dev, {B, Hkv, S}) ||
+            !optional_vector(arg[4], lens, B, dev) || !int_arg(arg[5], kv_len, 0) || !scale_arg(arg[6], scale))
+            Py_RETURN_NONE;
+        const c10::cuda::CUDAGuard guard(dev);
+        void* stream = stream_of(dev);
+        const int rc = unlocked([&] {
+            return rt_kv_weigh_bf16(ptr(q), ptr(k), ptr<float>(lse), ptr<float>(w), B, Hq, Hkv, T, (int)D, S, ptr<int32_t>(lens), kv_len,
+                                    scale, stream);
+        });
+        if (rc != RT_OK) Py_RETURN_NONE;
+        Py_RETURN_TRUE;
+    });
+}
+
+// The planes of either kind of cache for an eviction: four of a 4-bit cache, two of bf16.
+struct EvictArgs {
+    const Tensor* plane[4];
+    int n = 0;
+    int64_t B, Hkv, S, D;
+    at::Device dev = at::Device(at::kCPU);
+};
+inline bool evict_args(PyObject* o, EvictArgs& a) {
+    if (!PyTuple_Check(o)) return false;
+    if (PyTuple_GET_SIZE(o) == 4) {
+        Kv4Args c;
+        if (!kv4_args(o, c)) return false;
+        a.n = 4, a.B = c.B, a.Hkv = c.Hkv, a.S = c.S, a.D = c.D, a.dev = c.dev;
+        for (int i = 0; i < 4; ++i) a.plane[i] = c.plane[i];
+        return true;
+    }
+    if (PyTuple_GET_SIZE(o) != 2 || !(a.plane[0] = tensor_arg(PyTuple_GET_ITEM(o, 0))) || !(a.plane[1] = tensor_arg(PyTuple_GET_ITEM(o, 1))))
+        return false;
+    const Tensor& k = *a.plane[0];
+    if (!k.is_cuda() || k.dim() != 4) return false;
+    a.n = 2, a.dev = k.device(), a.B = k.size(0), a.Hkv = k.size(1), a.S = k.size(2), a.D = k.size(3);
+    return dense(k, kBf16, a.dev) && shaped(*a.plane[1], kBf16, a.dev, k.sizes());
+}
+
+// cache, out, weights, keep, recent, kv_lens, kv_len, weights_out -> (lens, weights_out, kept)
+PyObject* kv_evict(PyObject*, PyObject* const* arg, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        EvictArgs a, b;
+        if (n != 8 || !evict_args(arg[0], a) || !evict_args(arg[1], b)) Py_RETURN_NONE;
+        const Tensor *w = tensor_arg(arg[2]), *lens, *w_out;
+        int64_t keep, recent, kv_len;
+        if (a.n != b.n || a.B != b.B || a.Hkv != b.Hkv || a.D != b.D || a.dev != b.dev || !w ||
+            !shaped(*w, kF32, a.dev, {a.B, a.Hkv, a.S}) || !int_arg(arg[3], keep, -1) || !int_arg(arg[4], recent, 0) ||
+            !optional_vector(arg[5], lens, a.B, a.dev) || !int_arg(arg[6], kv_len, 0) || !optional_arg(arg[7], w_out) || keep < 1 ||
+            keep > b.S || (w_out && !shaped(*w_out, kF32, a.dev, {a.B, a.Hkv, b.S})))
+            Py_RETURN_NONE;
+        Tensor new_w;
+        if (!w_out) {
+            new_w = empty({a.B, a.Hkv, b.S}, kF32, a.dev);
+            w_out = &new_w;
+        }
+        const Tensor kept = empty({a.B, a.Hkv, keep}, at::kInt, a.dev), new_lens = empty({a.B}, at::kInt, a.dev);
+        const void* src[4] = {};
+        void* dst[4] = {};
+        int32_t bytes[4] = {};
+        for (int i = 0; i < a.n; ++i) {
+            src[i] = ptr(a.plane[i]), dst[i] = ptr(b.plane[i]);
+            bytes[i] = (int32_t)(a.n == 2 ? 2 * a.D : i % 2 ? a.D / 8 : a.D / 2);
+        }
+        const c10::cuda::CUDAGuard guard(a.dev);
+        void* stream = stream_of(a.dev);
+        const int rc = unlocked([&] {
+            return rt_kv_evict(src, dst, bytes, a.n, ptr<float>(w), ptr<float>(w_out), ptr<int32_t>(&kept), ptr<int32_t>(&new_lens), a.B,
+                               a.Hkv, a.S, b.S, ptr<int32_t>(lens), kv_len, keep, recent, stream);
+        });
+        if (rc != RT_OK) Py_RETURN_NONE;
+        return Py_BuildValue("(NNN)", THPVariable_Wrap(new_lens), THPVariable_Wrap(*w_out), THPVariable_Wrap(kept));
+    });
+}
+
 #define RT_METHOD(name, fn) {name, (PyCFunction)(void (*)(void))(fn), METH_FASTCALL, nullptr}
 PyMethodDef kMethods[] = {
     RT_METHOD("gqa_decode", gqa_decode),
@@ -398,6 +651,12 @@ PyMethodDef kMethods[] = {
     RT_METHOD("prefill_f32", prefill_f32),
     RT_METHOD("backward_f32", backward<false>),
     RT_METHOD("backward_bf16", backward<true>),
+    RT_METHOD("kv4_append", kv4_append),
+    RT_METHOD("rope_kv4_append", rope_kv4_append),
+    RT_METHOD("kv4_read", kv4_read),
+    RT_METHOD("kv4_decode", kv4_decode),
+    RT_METHOD("kv_weigh", kv_weigh),
+    RT_METHOD("kv_evict", kv_evict),
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_torch_binding", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};

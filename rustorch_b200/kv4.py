@@ -85,6 +85,8 @@ def kv4_append(cache: Kv4Cache, k, v, pos: Optional[int] = None, positions=None,
     and whose strides are multiples of 8, e.g. a projection's ``[B, T, Hkv, D]`` permuted.  Row i goes to position ``pos`` + i
     (default 0) of every sequence, or ``positions[b]`` + i (int32 CUDA ``[B]``; rows outside the cache are dropped then).
     ``lens``: optional int32 CUDA ``[B]``, how many rows of each sequence count.  Enqueues on the current stream."""
+    if type(cache) is Kv4Cache and (_lib._binding or _lib.torch_binding()).kv4_append(cache, k, v, pos, positions, lens):
+        return
     import torch
     B, Hkv, S, D = _guard_cache(cache)
     ptrs, strides = [], []
@@ -114,6 +116,9 @@ def rope_kv4_append(q, k_in, v_in, cache: Kv4Cache, inv_freq, pos: Optional[int]
     """Rotary embedding of q (in place) and of the new K row, and append of K and V to a 4-bit cache, one launch
     (``rt_rope_kv4_append``).  q ``[B,Hq,D]``, k_in, v_in ``[B,Hkv,D]`` as for ``rope_kv_append``.  The rows go to the rotary
     position, or to ``slot`` / ``slots`` (int32 CUDA ``[B]``) where a cache's rows and positions have come apart."""
+    if type(cache) is Kv4Cache and (_lib._binding or _lib.torch_binding()).rope_kv4_append(
+            q, k_in, v_in, cache, inv_freq, pos, positions, slot, slots, _ROPE_STYLES[style]):
+        return
     import torch
     B, Hkv, S, D = _guard_cache(cache)
     _guard("q", q, torch.bfloat16, like=cache.k_codes)
@@ -136,6 +141,10 @@ def kv4_read(cache: Kv4Cache, rows: int, start: int = 0, starts=None, kv_lens=No
     """Rows of the cache in bf16 via ``rt_kv4_read``: (k, v) ``[B, Hkv, rows, D]``, row i being the cache's row ``start`` + i
     or ``starts[b]`` + i (int32 CUDA ``[B]``), and zero from ``kv_lens[b]`` (int32 CUDA ``[B]``; default: the cache's end) on.
     ``out``: optional pair of tensors to write."""
+    if type(cache) is Kv4Cache:
+        r = (_lib._binding or _lib.torch_binding()).kv4_read(cache, rows, start, starts, kv_lens, out)
+        if r is not None:
+            return r
     import torch
     B, Hkv, S, D = _guard_cache(cache)
     rows = int(rows)
@@ -166,6 +175,11 @@ def kv4_decode(q, cache: Kv4Cache, kv_lens=None, kv_len: Optional[int] = None, s
     (out bf16 ``[B,Hq,D]``, lse f32 ``[B,Hq]`` or None); both may be passed in.  ``weights``: optional f32 ``[B,Hkv,max_seq]``
     to which every token's softmax weight, summed over the query heads of its KV head, is added.  ``workspace``: optional
     uint8 CUDA tensor of ``kv4_workspace_bytes(...)`` bytes; two calls that overlap on the GPU need one each."""
+    if type(cache) is Kv4Cache:
+        r = (_lib._binding or _lib.torch_binding()).kv4_decode(q, cache, kv_lens, kv_len, scale, return_lse, weights, workspace, out,
+                                                               lse)
+        if r is not None:
+            return r
     import torch
     B, Hkv, S, D = _guard_cache(cache)
     _guard("q", q, torch.bfloat16, like=cache.k_codes)

@@ -392,3 +392,46 @@ def test_steps_of_a_token_loop(rt):
         got, got_lse = rt.kv4_decode(qs, cache, kv_lens=lens)
         _check(got, o, ot, "out")
         _check(got_lse, l, lt, "lse")
+
+
+# ------------------------------------------------------------------------------------------------ the two paths to the entries
+
+
+class _Nothing:
+    """Stands in for the extension and covers nothing."""
+    def __getattr__(self, name):
+        return lambda *args: None
+
+
+def _every_call(rt):
+    B, Hq, Hkv, D, S = 2, 8, 2, 64, 100
+    lens, at = _i32(90, 13), _i32(95, 14)
+    q, k, v = _randn(B, Hq, D, seed=1), _randn(B, Hkv, D, seed=2), _randn(B, Hkv, D, seed=3)
+    cache = plain.fill(rt, B, Hkv, S, D, 4)
+    rt.kv4_append(cache, k, v, pos=2)
+    rt.kv4_append(cache, *(_randn(B, 5, Hkv, D, seed=i).transpose(1, 2) for i in (5, 6)), positions=_i32(20, 99), lens=_i32(5, 1))
+    rt.rope_kv4_append(q, k, v, cache, rt.rope_inv_freq(D), positions=at, slot=40, style="adjacent")
+    rt.rope_kv4_append(q, k, v, cache, rt.rope_inv_freq(D), pos=7, slots=at)
+    weights, ws = torch.zeros(B, Hkv, S, device="cuda"), torch.zeros(1 << 22, dtype=torch.uint8, device="cuda")
+    out, lse = rt.kv4_decode(q, cache, kv_lens=lens, weights=weights, scale=0.2, workspace=ws)
+    out2, none = rt.kv4_decode(q, cache, kv_len=77, return_lse=False, out=torch.empty_like(q))
+    assert none is None
+    kb, vb = rt.kv4_read(cache, S)
+    k2, v2 = rt.kv4_read(cache, 9, starts=at, kv_lens=lens, out=(torch.empty(B, Hkv, 9, D, dtype=torch.bfloat16, device="cuda"),) * 2)
+    _, l16 = rt.gqa_decode(q, kb, vb, kv_lens=lens)
+    rt.kv_weigh(q, kb, l16, weights, kv_lens=lens)
+    rt.kv_weigh(q[:, :, None].expand(B, Hq, 3, D).contiguous(), kb, l16[:, :, None].expand(B, Hq, 3).contiguous(), weights, kv_len=50)
+    small, pair = rt.Kv4Cache.new(B, Hkv, 30, D), (torch.zeros(B, Hkv, 30, D, dtype=torch.bfloat16, device="cuda"),
+                                                  torch.zeros(B, Hkv, 30, D, dtype=torch.bfloat16, device="cuda"))
+    evicted = rt.kv_evict(cache, small, weights, 20, recent=3, kv_lens=lens)
+    evicted += rt.kv_evict((kb, vb), pair, weights, 25, kv_len=100, weights_out=torch.ones(B, Hkv, 30, device="cuda"))
+    return [q, *cache, weights, out, lse, out2, kb, vb, k2, *small, *pair, *evicted]
+
+
+def test_extension_and_ctypes_paths_agree(rt, monkeypatch):
+    from rustorch_b200 import _lib
+    got = _every_call(rt)
+    monkeypatch.setattr(_lib, "_binding", _Nothing())
+    want = _every_call(rt)
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype and a.shape == b.shape and torch.equal(a, b)
