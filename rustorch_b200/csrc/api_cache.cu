@@ -12,7 +12,7 @@ inline float default_scale(float scale, int dim) { return scale > 0.f ? scale : 
 inline bool head_dim_ok(int d) { return d == 64 || d == 128 || d == 256; }
 
 // Lengths and counts are 32-bit in the kernels, places in a tensor 64-bit.
-constexpr int64_t kMostSeq = 0x7fffff00;
+constexpr int64_t kMostSeq = 0x7fff0000;
 
 // The planes of a 4-bit cache: there and aligned.
 inline int check_planes(const rt::Kv4Cache& c) {
@@ -52,8 +52,7 @@ int rt_kv4_append(void* k_codes, void* k_scales, void* v_codes, void* v_scales, 
     if (!k || !v) return RT_ERR_NULL_POINTER;
     if (const int rc = check_planes(c)) return rc;
     if (!aligned16(k) || !aligned16(v)) return RT_ERR_ALIGNMENT;
-    // a CTA takes 8 rows at least
-    if (rows > kMostSeq || batch * n_kv > INT64_MAX / rows || batch * n_kv * rows > (int64_t)0x7fffffff * 8) return RT_ERR_UNSUPPORTED;
+    if (rows > kMostSeq) return RT_ERR_UNSUPPORTED;
     const int64_t dense[3] = {n_kv * rows * head_dim, rows * head_dim, head_dim};
     const int64_t *ks = k_strides ? k_strides : dense, *vs = v_strides ? v_strides : dense;
     for (int i = 0; i < 3; ++i)
@@ -91,9 +90,7 @@ int rt_kv4_read(const void* k_codes, const void* k_scales, const void* v_codes, 
     if (!k_out || !v_out) return RT_ERR_NULL_POINTER;
     if (const int rc = check_planes(c)) return rc;
     if (!aligned16(k_out) || !aligned16(v_out)) return RT_ERR_ALIGNMENT;
-    if (rows > kMostSeq || start > kMostSeq || start < -kMostSeq || batch * n_kv > INT64_MAX / rows ||
-        batch * n_kv * rows > (int64_t)0x7fffffff * 8)
-        return RT_ERR_UNSUPPORTED;
+    if (rows > kMostSeq || start > kMostSeq || start < -kMostSeq) return RT_ERR_UNSUPPORTED;
     return (int)rt::launch_kv4_read(c, k_out, v_out, batch, n_kv, head_dim, max_seq, rows, start, starts, kv_lens,
                                     as_stream(stream));
 }

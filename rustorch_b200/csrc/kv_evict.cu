@@ -1,4 +1,10 @@
 // Eviction from a KV cache: which rows stay (the heaviest and the latest), then their move to another cache.
+//
+// Selection: the weight of the last row that stays is found digit by digit (11, 11 and 10 bits of an order-preserving
+// integer), by histograms in shared memory; a scan in order then gives every kept row its place.  A cluster of 1 to 8 CTAs
+// shares the candidates of a (sequence, KV head): each has an equal run of them in its shared memory, reads the others'
+// histograms and counts there, and touches global memory once.  No order of atomics reaches the result: the histograms
+// are sums.
 #include <algorithm>
 
 #include "cache_kernels.h"
@@ -8,7 +14,9 @@
 namespace rt {
 namespace {
 
-constexpr int kThreads = 1024, kBins = 2048;
+constexpr int kThreads = 1024, kWarps = kThreads / 32, kBins = 2 * kThreads, kPasses = 3;
+constexpr int kMostCluster = 8;
+constexpr int kHeld = 32 * 1024;  // candidates of a CTA that its shared memory holds; longer runs are read again instead
 
 struct SelectParams {
     const float* weights;
@@ -16,8 +24,26 @@ struct SelectParams {
     int32_t *kept, *lens_out;
     int64_t max_seq, max_seq_out;
     const int32_t* kv_lens;
-    int kv_len, n_kv, keep, recent;
+    int kv_len, n_kv, keep, recent, cluster, held;  // held: candidates that the launch has shared memory for
 };
+
+struct SelectShared {
+    uint32_t bins[kPasses][kBins];
+    uint32_t larger, equal;  // of this CTA's candidates
+    uint64_t warps[kWarps];
+    uint32_t digit, above;
+};
+
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// What lies at `p` in the shared memory of the cluster's CTA `rank`.
+__device__ __forceinline__ uint32_t load_remote(const uint32_t* p, int rank) {
+    uint32_t at, x;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+    return x;
+}
 
 // A key that orders floats as unsigned integers, -0 as 0 and every NaN above infinity.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -26,96 +52,120 @@ __device__ __forceinline__ uint32_t order_key(float w) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Inclusive sum over the CTA; `total` the sum of all.
-__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t* warps, uint32_t& total) {
+// Inclusive sum over the CTA.
+__device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* warps) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-        const uint32_t y = __shfl_up_sync(kFullMask, x, off);
+        const uint64_t y = __shfl_up_sync(kFullMask, x, off);
         if (lane >= off) x += y;
     }
     __syncthreads();
     if (lane == 31) warps[warp] = x;
     __syncthreads();
-    uint32_t before = 0, all = 0;
-    for (int i = 0; i < kThreads / 32; ++i) {
-        const uint32_t y = warps[i];
-        before += i < warp ? y : 0;
-        all += y;
-    }
-    total = all;
+    static_assert(kWarps == 32, "a warp adds up the warps' sums");
+    uint64_t before = lane < warp ? warps[lane] : 0;
+#pragma unroll
+    for (int off = 16; off; off >>= 1) before += __shfl_xor_sync(kFullMask, before, off);
     return x + before;
 }
 
-// One CTA a (sequence, KV head): the want-th largest key by its digits of 11, 11 and 10 bits, then one pass in order.
 __global__ void __launch_bounds__(kThreads) kv_select_kernel(const SelectParams p) {
-    __shared__ uint32_t bins[kBins], warps[kThreads / 32], s_digit, s_above;
+    extern __shared__ __align__(16) uint8_t smem[];
+    SelectShared& sh = *reinterpret_cast<SelectShared*>(smem);
+    float* held = reinterpret_cast<float*>(smem + sizeof(SelectShared));
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int tid = threadIdx.x;
-    const int64_t b = blockIdx.y, bh = b * p.n_kv + blockIdx.x;
+    const int tid = threadIdx.x, C = p.cluster, rank = blockIdx.x % C, h = blockIdx.x / C;
+    const int64_t b = blockIdx.y, bh = b * p.n_kv + h;
     const int len = (int)max((int64_t)0, min(p.kv_lens ? (int64_t)p.kv_lens[b] : (int64_t)p.kv_len, p.max_seq));
     const int m = min(len, p.keep);
     const float* w = p.weights + bh * p.max_seq;
     float* w_out = p.weights_out + bh * p.max_seq_out;
     int32_t* kept = p.kept + bh * p.keep;
+    const int every = C * kThreads, mine = rank * kThreads + tid;
     if (blockIdx.x == 0 && tid == 0) p.lens_out[b] = m;
-    for (int i = m + tid; i < p.keep; i += kThreads) kept[i] = -1;
-    for (int64_t i = m + tid; i < p.max_seq_out; i += kThreads) w_out[i] = 0.f;
+    for (int i = m + mine; i < p.keep; i += every) kept[i] = -1;
+    for (int64_t i = m + mine; i < p.max_seq_out; i += every) w_out[i] = 0.f;
     if (len <= p.keep) {
-        for (int i = tid; i < len; i += kThreads) kept[i] = i, w_out[i] = w[i];
-        return;
+        for (int i = mine; i < len; i += every) kept[i] = i, w_out[i] = w[i];
+        return;  // the whole cluster does
     }
     const int n = len - p.recent;        // candidates
     const int want = p.keep - p.recent;  // of which so many stay
+    for (int i = mine; i < p.recent; i += every) kept[want + i] = n + i, w_out[want + i] = w[n + i];
+    if (want == 0) return;
+    // this CTA's run of them
+    const int run = (n + C - 1) / C, first = min(n, rank * run), count = min(n, first + run) - first;
+    const float* x = w + first;
+    for (int i = tid; i < kPasses * kBins; i += kThreads) sh.bins[0][i] = 0;
+    if (run <= p.held) {
+        for (int i = tid; i < count; i += kThreads) held[i] = x[i];
+        x = held;
+    }
+    __syncthreads();
     uint32_t prefix = 0, mask = 0;
     int left = want;  // of the candidates with the prefix
-    if (want > 0) {
-        const int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = shifts[pass];
-            const uint32_t digit = (1u << widths[pass]) - 1;
-            for (int i = tid; i < kBins; i += kThreads) bins[i] = 0;
-            __syncthreads();
-            for (int i = tid; i < n; i += kThreads) {
-                const uint32_t k = order_key(w[i]);
-                if ((k & mask) == prefix) atomicAdd(&bins[k >> shift & digit], 1u);
-            }
-            __syncthreads();
-            // the digit where the count from above reaches `left`: thread i holds bins 2i and 2i+1 from the top
-            const uint32_t hi_bin = kBins - 1 - 2 * tid, a = bins[hi_bin], c = bins[hi_bin - 1];
-            uint32_t total;
-            const uint32_t upto = block_scan(a + c, warps, total), before = upto - a - c;
-            if (before < (uint32_t)left && upto >= (uint32_t)left) {
-                const bool first = before + a >= (uint32_t)left;
-                s_digit = first ? hi_bin : hi_bin - 1;
-                s_above = first ? before : before + a;
-            }
-            __syncthreads();
-            prefix |= s_digit << shift;
-            mask |= digit << shift;
-            left -= (int)s_above;
-            __syncthreads();
+#pragma unroll
+    for (int pass = 0; pass < kPasses; ++pass) {
+        constexpr int shifts[kPasses] = {21, 10, 0}, widths[kPasses] = {11, 11, 10};
+        const int shift = shifts[pass];
+        const uint32_t digit = (1u << widths[pass]) - 1;
+        uint32_t* bins = sh.bins[pass];
+        for (int i = tid; i < count; i += kThreads) {
+            const uint32_t k = order_key(x[i]);
+            if ((k & mask) == prefix) atomicAdd(&bins[k >> shift & digit], 1u);
         }
-        // in order: larger keys, and the first `left` equal ones
-        uint32_t larger = 0, equal = 0;
-        for (int i0 = 0; i0 < n; i0 += kThreads) {
-            const int i = i0 + tid;
-            const float x = i < n ? w[i] : 0.f;
-            const uint32_t k = order_key(x);
-            const bool gt = i < n && k > prefix, eq = i < n && k == prefix;
-            uint32_t total;
-            const uint32_t at = block_scan((uint32_t)gt | (uint32_t)eq << 16, warps, total);
-            const uint32_t gt_before = larger + (at & 0xffffu) - gt, eq_before = equal + (at >> 16) - eq;
-            if (gt || (eq && eq_before < (uint32_t)left)) {
-                const uint32_t to = gt_before + min(eq_before, (uint32_t)left);
-                kept[to] = i, w_out[to] = x;
-            }
-            larger += total & 0xffffu, equal += total >> 16;
+        if (C > 1) cluster_barrier();
+        else __syncthreads();
+        // the digit where the count from above reaches `left`: thread i holds bins 2i and 2i + 1 from the top
+        const uint32_t hi_bin = kBins - 1 - 2 * tid;
+        uint32_t a = 0, c = 0;
+        if (C > 1) {
+            for (int r = 0; r < C; ++r) a += load_remote(&bins[hi_bin], r), c += load_remote(&bins[hi_bin - 1], r);
+        } else {
+            a = bins[hi_bin], c = bins[hi_bin - 1];
         }
+        const uint32_t upto = (uint32_t)block_scan(a + c, sh.warps), before = upto - a - c;
+        if (before < (uint32_t)left && upto >= (uint32_t)left) {
+            const bool upper = before + a >= (uint32_t)left;
+            sh.digit = upper ? hi_bin : hi_bin - 1;
+            sh.above = upper ? before : before + a;
+        }
+        __syncthreads();
+        prefix |= sh.digit << shift;
+        mask |= digit << shift;
+        left -= (int)sh.above;
     }
-    for (int i = tid; i < p.recent; i += kThreads) kept[want + i] = n + i, w_out[want + i] = w[n + i];
+    // In order: larger keys, and the first `left` equal ones.  A thread has an odd number of neighbours, so that a warp's
+    // reads lie in different banks.
+    const int each = ((count + kThreads - 1) / kThreads) | 1;
+    const int begin = min(count, tid * each), end = min(count, begin + each);
+    uint32_t gt = 0, eq = 0;
+    for (int i = begin; i < end; ++i) {
+        const uint32_t k = order_key(x[i]);
+        gt += k > prefix, eq += k == prefix;
+    }
+    const uint64_t upto = block_scan((uint64_t)gt << 32 | eq, sh.warps);
+    gt = (uint32_t)(upto >> 32) - gt, eq = (uint32_t)upto - eq;  // of the threads before
+    if (C > 1) {
+        if (tid == kThreads - 1) sh.larger = (uint32_t)(upto >> 32), sh.equal = (uint32_t)upto;
+        cluster_barrier();
+        for (int r = 0; r < rank; ++r) gt += load_remote(&sh.larger, r), eq += load_remote(&sh.equal, r);
+    }
+    for (int i = begin; i < end; ++i) {
+        const float v = x[i];
+        const uint32_t k = order_key(v);
+        if (k > prefix || (k == prefix && eq < (uint32_t)left)) {
+            const uint32_t to = gt + min(eq, (uint32_t)left);
+            kept[to] = first + i, w_out[to] = v;
+        }
+        gt += k > prefix, eq += k == prefix;
+    }
+    if (C > 1) cluster_barrier();  // nobody leaves while its shared memory is read
 }
+
+constexpr int kMoveRows = 64, kMoveThreads = 256;
 
 struct MoveParams {
     EvictPlanes planes;
@@ -124,19 +174,44 @@ struct MoveParams {
     int keep;
 };
 
-// 8 bytes a thread and step; grid: (rows, plane, sequence and head).
-__global__ void __launch_bounds__(256) kv_move_kernel(const MoveParams p) {
+// 64 kept rows of a (sequence, KV head), all planes.
+template <class Unit>
+__device__ __forceinline__ void move_rows(const uint8_t* src, uint8_t* dst, const int32_t* from, int rows, int row_bytes) {
+    const unsigned units = row_bytes / sizeof(Unit), all = rows * units;
+    constexpr int kBatch = 4;  // loads of a thread in flight
+    for (unsigned i0 = threadIdx.x; i0 < all; i0 += kBatch * kMoveThreads) {
+        Unit x[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const unsigned i = i0 + k * kMoveThreads, r = i / units;
+            if (i < all) x[k] = *reinterpret_cast<const Unit*>(src + (int64_t)from[r] * row_bytes + (i - r * units) * sizeof(Unit));
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const unsigned i = i0 + k * kMoveThreads;
+            if (i < all) *reinterpret_cast<Unit*>(dst + (int64_t)i * sizeof(Unit)) = x[k];
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const MoveParams p) {
+    __shared__ int32_t from[kMoveRows];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t bh = blockIdx.z;
-    const int plane = blockIdx.y, units = p.planes.row_bytes[plane] / 8;
-    const uint2* src = static_cast<const uint2*>(p.planes.src[plane]) + bh * p.max_seq * units;
-    uint2* dst = static_cast<uint2*>(p.planes.dst[plane]) + bh * p.max_seq_out * units;
-    const int32_t* kept = p.kept + bh * p.keep;
-    const int64_t all = (int64_t)p.keep * units;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / units, from = kept[row];
-        if (from >= 0) dst[i] = src[from * units + i % units];
+    const int64_t bh = blockIdx.y;
+    const int first = blockIdx.x * kMoveRows, most = min(kMoveRows, p.keep - first);
+    bool there = false;
+    if (threadIdx.x < most) {
+        from[threadIdx.x] = p.kept[bh * p.keep + first + threadIdx.x];
+        there = from[threadIdx.x] >= 0;
+    }
+    const int rows = __syncthreads_count(there);  // those behind the kept ones come last
+    for (int i = 0; i < p.planes.n; ++i) {
+        const int bytes = p.planes.row_bytes[i];
+        const uint8_t* src = static_cast<const uint8_t*>(p.planes.src[i]) + bh * p.max_seq * bytes;
+        uint8_t* dst = static_cast<uint8_t*>(p.planes.dst[i]) + (bh * p.max_seq_out + first) * bytes;
+        if (bytes % 16 == 0) move_rows<uint4>(src, dst, from, rows, bytes);
+        else move_rows<uint2>(src, dst, from, rows, bytes);
     }
 }
 
@@ -150,14 +225,34 @@ cudaError_t launch_kv_evict(const EvictPlanes& planes, const float* weights, flo
     s.weights = weights, s.weights_out = weights_out, s.kept = kept, s.lens_out = lens_out;
     s.max_seq = max_seq, s.max_seq_out = max_seq_out, s.kv_lens = kv_lens, s.kv_len = (int)kv_len_uniform;
     s.n_kv = n_kv, s.keep = (int)keep, s.recent = (int)recent;
-    cudaError_t e = launch_chained(kv_select_kernel, dim3(n_kv, (unsigned)batch), kThreads, 0, stream, s);
+    // More CTAs a head while each keeps 2048 candidates and all find an SM.
+    const int64_t longest = kv_lens ? max_seq : kv_len_uniform;
+    int cluster = 1;
+    while (cluster < kMostCluster && longest >= 2 * cluster * 2048 && 2 * cluster * batch * n_kv <= sm_count()) cluster *= 2;
+    s.cluster = cluster;
+    const int64_t run = (longest + cluster - 1) / cluster;
+    s.held = run <= kHeld ? (int)run : 0;
+    const size_t smem = sizeof(SelectShared) + s.held * sizeof(float);
+    cudaError_t e = set_max_dynamic_smem_once<kv_select_kernel>((int)sizeof(SelectShared) + kHeld * (int)sizeof(float));
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(n_kv * cluster), (unsigned)batch);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, kv_select_kernel, s);
     if (e != cudaSuccess) return e;
     MoveParams m;
     m.planes = planes, m.kept = kept, m.max_seq = max_seq, m.max_seq_out = max_seq_out, m.keep = (int)keep;
-    int units = 1;
-    for (int i = 0; i < planes.n; ++i) units = max(units, planes.row_bytes[i] / 8);
-    const unsigned x = (unsigned)min((int64_t)256, (keep * units + 1023) / 1024);
-    return launch_chained(kv_move_kernel, dim3(x, planes.n, (unsigned)(batch * n_kv)), 256, 0, stream, m);
+    return launch_chained(kv_move_kernel, dim3((unsigned)((keep + kMoveRows - 1) / kMoveRows), (unsigned)(batch * n_kv)), kMoveThreads,
+                          0, stream, m);
 }
 
 }  // namespace rt
