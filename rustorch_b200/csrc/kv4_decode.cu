@@ -1,10 +1,11 @@
 // Single-token GQA attention over a 4-bit KV cache.
 //
 // out = sum_t p_t v_t, p = softmax(scale * q . k_t), with k, v = lo + scale * code per group of 32 values.  Per group
-//     q . k = scale * sum(q * code) + lo * sum(q),        sum_t p_t v_t = sum_t (p_t scale_t) code_t + sum_t p_t lo_t,
-// so the matrix instructions run on the bare codes and nothing is dequantised.  A code in the low bits of a 16-bit half is
-// the f16 subnormal code * 2^-24, which mma.sync multiplies exactly: one AND makes a pair of operands, and the high
-// nibble of a byte, 16 times as large, is met by a q (or a result row) that is 16 times as small.
+//     q . k = scale * sum(q * code) + lo * sum(q),        sum_t p_t v_t = sum_t p_t (scale_t code_t) + sum_t p_t lo_t.
+// A code in the low bits of a 16-bit half is the f16 subnormal code * 2^-24, which mma.sync multiplies exactly: one AND makes
+// a pair of operands, and the high nibble of a byte, 16 times as large, is met by a q (or a result row) that is 16 times
+// as small.  Keys need nothing else: the scale goes onto the 16 x 8 products.  Of V a product sums over tokens, so the
+// scale goes onto the codes (an f16 product, rounded to 11 bits).
 #include <algorithm>
 
 #include "cache_kernels.h"
@@ -42,7 +43,7 @@ struct DecodeParams {
     __nv_bfloat16* out;
     float* lse;
     float* weights;
-    float* scores;   // [B * Hkv, max_seq, group] scaled scores (log2), where weights are asked for
+    float* scores;   // [B * Hq, max_seq] scaled scores (log2), where weights are asked for
     float* part_o;   // [2 * CTAs][group][D]
     float2* part_ml; // [2 * CTAs][group]: the reference that the part's sums are relative to (log2), the sum of its weights
     int64_t max_seq;
@@ -202,15 +203,25 @@ struct Queries {
 // What a warp has summed so far.  Lane (g, j) holds queries 2j and 2j + 1.
 template <int D>
 struct Sums {
-    float o[Shape<D>::kGroups][2][4];  // [group][dims 0-1, 2-3 of a lane's four]: codes, {q 2j, 2j+1} x {even, odd dim}
-    float lo[4];                       // sum p * lo, row g = group g
-    float ref[2], top[2], l[2];        // p = 2^(score - ref); running maximum; sum of p (this lane's tokens)
+    float o[D / 32][2][4];       // [32 dims][0-1, 2-3 of a lane's four]: sum p scale code 2^(k - 24), {q 2j, 2j+1} x {even, odd dim}
+    float lo[4];                 // sum p * lo, row g = its group
+    float ref[2], top[2], l[2];  // p = 2^(score - ref); running maximum; sum of p (this lane's tokens)
+    int k;                       // scales are held times 2^k: the largest so far lies in [2^14, 2^15)
+    uint32_t scale_limit;        // the largest f16 pattern for which k stands
 };
+constexpr float kBase = 15.f - kLazy;  // log2 of what p is held times: the largest reaches 2^15
 
-// 32 tokens (valid of them) that lie in shared memory.
+__device__ __forceinline__ void load_transposed(uint32_t (&r)[4], uint32_t at) {  // four 8x8 matrices of 16-bit values
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(at)
+                 : "memory");
+}
+
+// 32 tokens (valid of them) that lie in shared memory.  scores: [query][max_seq] from this step's first token on, or null.
 template <int D>
-__device__ __forceinline__ void step(const uint8_t* stage, int valid, const Queries<D>& q, Sums<D>& a, float& base,
-                                     uint32_t& scale_limit, int lane, float* scores, int group) {
+__device__ __forceinline__ void step(const uint8_t* stage, int valid, const Queries<D>& q, Sums<D>& a, int lane, float* scores,
+                                     int64_t max_seq, int group) {
     using S = Shape<D>;
     const int g = lane / 4, j = lane % 4;
     const uint8_t *kc = stage, *vc = stage + S::kKBytes, *ks = vc + S::kVBytes, *vs = ks + S::kScaleBytes;
@@ -260,17 +271,19 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
             for (int k = 0; k < 4; ++k)
                 if (tb * 16 + g + 4 * (k & 2) >= valid) x[tb][k] = -INFINITY;
     }
-    if (scores) {  // [token][query]
+    if (scores) {
 #pragma unroll
-        for (int tb = 0; tb < 2; ++tb)
+        for (int c = 0; c < 2; ++c)
+            if (2 * j + c < group) {
+                float* row = scores + (2 * j + c) * max_seq;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int t = tb * 16 + g + 4 * (k & 2), h = 2 * j + (k & 1);
-                if (t < valid && h < group) scores[t * group + h] = x[tb][k];
+                for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r)
+                        if (tb * 16 + 8 * r + g < valid) row[tb * 16 + 8 * r + g] = x[tb][2 * r + c];
             }
     }
-    // The largest scale of V's 32 tokens: p is held times 2^base so that p * scale stays within f16.
-    uint32_t big = 0;
+    uint32_t big = 0;  // the largest scale of V: each lane looks at a token
 #pragma unroll
     for (int i = 0; i < S::kGroups; i += S::kSpanGroups) {
         uint32_t w[S::kSpanGroups];
@@ -286,30 +299,34 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
         m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 8));
         top[c] = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16));
     }
-    if (__any_sync(kFullMask, top[0] > a.top[0] + kLazy || top[1] > a.top[1] + kLazy || big > scale_limit)) {
+    if (__any_sync(kFullMask, top[0] > a.top[0] + kLazy || top[1] > a.top[1] + kLazy || big > a.scale_limit)) {
         big = __reduce_max_sync(kFullMask, big);
-        if (big > scale_limit) {  // s < 2^(exponent + 1)
-            scale_limit = big | 0x3ffu;
-            base = 15.f - kLazy - (float)((int)(big >> 10) - 14);
+        float grow = 1.f;  // of the scales
+        if (big > a.scale_limit) {
+            const int e = (int)(__float_as_uint(low_half(big)) >> 23) - 127, k = 14 - e;
+            grow = exp2f((float)(k - a.k));
+            a.k = k;
+            a.scale_limit = (uint32_t)__half_as_ushort(__float2half_rn(exp2f((float)(e + 1)))) - 1;
         }
         float alpha[2];
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const bool first = a.top[c] == -INFINITY;
             a.top[c] = fmaxf(a.top[c], top[c]);
-            const float ref = a.top[c] == -INFINITY ? 0.f : a.top[c] - base;
+            const float ref = a.top[c] == -INFINITY ? 0.f : a.top[c] - kBase;
             alpha[c] = first ? 1.f : exp2f(a.ref[c] - ref);
             a.ref[c] = ref;
             a.l[c] *= alpha[c];
         }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a.lo[k] *= alpha[k & 1];
+        alpha[0] *= grow, alpha[1] *= grow;
 #pragma unroll
         for (int i = 0; i < S::kGroups; ++i)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) a.o[i][t][k] *= alpha[k & 1];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) a.lo[k] *= alpha[k & 1];
     }
     uint32_t prob[2][2];  // query g, tokens 2j, 2j + 1 (and 8 more) of a block of 16
 #pragma unroll
@@ -320,68 +337,82 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
             e[k] = fast_exp2(x[tb][k] - a.ref[k & 1]);
             a.l[k & 1] += e[k];
         }
-        // rounded to f16's 11 bits (once more with the token's scale), 2^-4 of the result's own rounding to bf16
+        // rounded to f16's 11 bits, an eighth of the result's own rounding to bf16
         prob[tb][0] = transposed(pack_half2(e[0], e[1]));
         prob[tb][1] = transposed(pack_half2(e[2], e[3]));
     }
-    const uint32_t half_of = (g & 1) ? 0x7632u : 0x5410u;
+    const float up = __uint_as_float((uint32_t)(127 + a.k) << 23);
+    // V transposed: unit u (4 codes of one token) of a row's 16 bytes goes to the lanes g = u, tokens 2j and 2j + 1 in one
+    // register.  Lane g's units belong to one group of each span.
+    const int own = (S::kSpanGroups == 4 ? g >> 1 : (g >> 1) & 1) * 4;
+    const uint32_t v_at = (uint32_t)__cvta_generic_to_shared(vc) + (lane & 15) * S::kVPitch + (lane >> 4) * 16;
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb) {
-        const int t = tb * 16 + 2 * j;
-        {  // sum p * lo: row g of the product is group g
-            const uint8_t* at = vs + t * S::kScaleRow + (g & (S::kGroups - 1)) * 4;
-            const uint32_t a0 = __byte_perm(*reinterpret_cast<const uint32_t*>(at), *reinterpret_cast<const uint32_t*>(at + S::kScaleRow), 0x7632),
-                           a2 = __byte_perm(*reinterpret_cast<const uint32_t*>(at + 8 * S::kScaleRow),
-                                            *reinterpret_cast<const uint32_t*>(at + 9 * S::kScaleRow), 0x7632);
-            mma_f16(a.lo, a0, 0u, a2, 0u, prob[tb][0], prob[tb][1]);
-        }
+        const uint8_t* at = vs + (tb * 16 + 2 * j) * S::kScaleRow + own;
 #pragma unroll
         for (int s = 0; s < S::kSpans; ++s) {
-            uint32_t w[4][S::kSpanGroups], f[4][S::kSpanGroups];
+            uint32_t f[4];  // {scale, lo} of tokens 2j, 2j + 1, 2j + 8, 2j + 9
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int row = t + (k & 1) + 4 * (k & 2);
-                load_words(w[k], vc + row * S::kVPitch + s * 64 + (g >> 1) * 4 * S::kSpanGroups);
-                load_words(f[k], vs + row * S::kScaleRow + s * 4 * S::kSpanGroups);
-            }
+            for (int k = 0; k < 4; ++k)
+                f[k] = *reinterpret_cast<const uint32_t*>(at + s * 4 * S::kSpanGroups + ((k & 1) + 4 * (k & 2)) * S::kScaleRow);
+            // sum p * lo: row g of the product is lane g's group, rows 8 and up of the second span
+            const uint32_t lo0 = __byte_perm(f[0], f[1], 0x7632), lo1 = __byte_perm(f[2], f[3], 0x7632);
+            if (s == 0) mma_f16(a.lo, lo0, 0u, lo1, 0u, prob[tb][0], prob[tb][1]);
+            else mma_f16(a.lo, 0u, lo0, 0u, lo1, prob[tb][0], prob[tb][1]);
+            const uint32_t s0 = pack_half2(low_half(f[0]) * up, low_half(f[1]) * up),
+                           s1 = pack_half2(low_half(f[2]) * up, low_half(f[3]) * up);
 #pragma unroll
-            for (int i = 0; i < S::kSpanGroups; ++i) {
-                const int gi = s * S::kSpanGroups + i;
-                const uint32_t b0 = mul_half2(prob[tb][0], __byte_perm(f[0][i], f[1][i], 0x5410)),
-                               b1 = mul_half2(prob[tb][1], __byte_perm(f[2][i], f[3][i], 0x5410));
-                uint32_t p0 = __byte_perm(w[0][i], w[1][i], half_of), p1 = __byte_perm(w[2][i], w[3][i], half_of);
-                mma_f16(a.o[gi][0], p0 & 0x000f000fu, p0 & 0x00f000f0u, p1 & 0x000f000fu, p1 & 0x00f000f0u, b0, b1);
-                p0 >>= 8, p1 >>= 8;
-                mma_f16(a.o[gi][1], p0 & 0x000f000fu, p0 & 0x00f000f0u, p1 & 0x000f000fu, p1 & 0x00f000f0u, b0, b1);
+            for (int i = 0; i < S::R::kSpan / 32; i += 2) {
+                const int gi = s * (S::R::kSpan / 32) + i;
+                uint32_t w[4];  // 32 dims, tokens 0-7 and 8-15; the next 32
+                load_transposed(w, v_at + tb * 16 * S::kVPitch + gi * 16);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t u0 = w[2 * c], u1 = w[2 * c + 1];
+                    mma_f16(a.o[gi + c][0], mul_half2(u0 & 0x000f000fu, s0), mul_half2(u0 & 0x00f000f0u, s0),
+                            mul_half2(u1 & 0x000f000fu, s1), mul_half2(u1 & 0x00f000f0u, s1), prob[tb][0], prob[tb][1]);
+                    u0 >>= 8, u1 >>= 8;
+                    mma_f16(a.o[gi + c][1], mul_half2(u0 & 0x000f000fu, s0), mul_half2(u0 & 0x00f000f0u, s0),
+                            mul_half2(u1 & 0x000f000fu, s1), mul_half2(u1 & 0x00f000f0u, s1), prob[tb][0], prob[tb][1]);
+                }
             }
         }
     }
 }
 
-// A warp's copies of 32 tokens from `from` on, `valid` of them, into a stage.
+// A lane's places in the planes: the step's bytes are contiguous, 16 neighbouring ones a lane and copy.
+struct LanePlanes {
+    const uint8_t *k, *v, *ks, *vs;
+};
+
+// A warp's copies of 32 tokens, `valid` of them, into a stage.  Rows behind them become zeros.
 template <int D>
-__device__ __forceinline__ void fetch(uint8_t* stage, const DecodeParams& p, int64_t row, int valid, int lane) {
+__device__ __forceinline__ void fetch(uint32_t to, const LanePlanes& from, int64_t token, int valid, int lane) {
     using S = Shape<D>;
-    const uint32_t to = (uint32_t)__cvta_generic_to_shared(stage);
     constexpr int kChunks = S::kRow / 16;  // of a row's codes
+    constexpr int kRows = 32 / kChunks;    // that a copy of the warp covers
+    constexpr int kPiece = S::kScaleRow < 16 ? S::kScaleRow : 16, kPieces = S::kScaleRow / kPiece;
+    const int r = lane / kChunks, c = lane % kChunks, r_scale = lane / kPieces;
+    // at D = 256 odd rows have their spans swapped
+    const uint32_t k_to = to + r * S::kRow + (S::kSpans == 2 ? c ^ ((r & 1) << 2) : c) * 16;
+    const uint32_t v_to = to + S::kKBytes + r * S::kVPitch + c * 16;
+    const uint32_t s_to = to + S::kKBytes + S::kVBytes + lane * kPiece;
+    const uint8_t *k = from.k + token * S::kRow, *v = from.v + token * S::kRow;
+    const uint8_t *ks = from.ks + token * S::kScaleRow, *vs = from.vs + token * S::kScaleRow;
+    static_assert(kRows % 2 == 0, "a row's parity is the same in all copies of a lane");
 #pragma unroll
     for (int n = 0; n < kChunks; ++n) {
-        const int x = lane + 32 * n, r = x / kChunks, c = x % kChunks;
-        const bool there = r < valid;
-        const int64_t from = (row + (there ? r : 0)) * S::kRow + c * 16;
-        const int swapped = S::kSpans == 2 ? c ^ ((r & 1) << 2) : c;
-        copy_async<16>(to + r * S::kRow + swapped * 16, p.k_codes + from, there);
-        copy_async<16>(to + S::kKBytes + r * S::kVPitch + c * 16, p.v_codes + from, there);
+        const bool there = valid >= kStep || r + n * kRows < valid;
+        const int64_t at = there ? n * 512 : 0;
+        copy_async<16>(k_to + n * kRows * S::kRow, there ? k + at : from.k - lane * 16, there);
+        copy_async<16>(v_to + n * kRows * S::kVPitch, there ? v + at : from.v - lane * 16, there);
     }
-    constexpr int kPiece = S::kScaleRow < 16 ? S::kScaleRow : 16, kPieces = S::kScaleRow / kPiece;
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) {
-        const int x = lane + 32 * n, r = x / kPieces, c = x % kPieces;
-        const bool there = r < valid;
-        const int64_t from = (row + (there ? r : 0)) * S::kScaleRow + c * kPiece;
-        const uint32_t at = to + S::kKBytes + S::kVBytes + r * S::kScaleRow + c * kPiece;
-        copy_async<kPiece>(at, p.k_scales + from, there);
-        copy_async<kPiece>(at + S::kScaleBytes, p.v_scales + from, there);
+        const bool there = valid >= kStep || r_scale + n * (32 / kPieces) < valid;
+        const int64_t at = there ? n * 32 * kPiece : 0;
+        copy_async<kPiece>(s_to + n * 32 * kPiece, there ? ks + at : from.ks - lane * kPiece, there);
+        copy_async<kPiece>(s_to + S::kScaleBytes + n * 32 * kPiece, there ? vs + at : from.vs - lane * kPiece, there);
     }
 }
 
@@ -424,6 +455,9 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
         }
     }
     uint8_t* ring = smem + warp * kStages * S::kStage;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    constexpr int kPiece = S::kScaleRow < 16 ? S::kScaleRow : 16;
+    const LanePlanes planes{p.k_codes + lane * 16, p.v_codes + lane * 16, p.k_scales + lane * kPiece, p.v_scales + lane * kPiece};
     for (bool head = true; at < end; head = false) {
         const int len = visible(p, b), n = tiles_of(len);
         const int h = (int)((at - first) / n), tile = (int)((at - first) % n);
@@ -433,7 +467,10 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
         const bool whole = tiles == n;
         const int steps = (hi - lo + kStep - 1) / kStep;  // of the CTA; 0 without tokens
         auto prefetch = [&](int s, int slot) {
-            if (s < steps) fetch<D>(ring + slot * S::kStage, p, rows + lo + s * kStep, min(kStep, hi - lo - s * kStep), lane);
+            const int valid = hi - lo - s * kStep;
+            const uint32_t to = ring_at + slot * S::kStage;
+            if (valid >= kStep) fetch<D>(to, planes, rows + lo + s * kStep, kStep, lane);  // compiled without the tests
+            else if (valid > 0) fetch<D>(to, planes, rows + lo + s * kStep, valid, lane);
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 #pragma unroll
@@ -442,8 +479,6 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
         q.load(p, bh, lane);
         Sums<D> a = {};
         a.top[0] = a.top[1] = -INFINITY;
-        float base = 15.f - kLazy;
-        uint32_t scale_limit = 0x3bffu;  // scales below 1
         int slot = 0;
         for (int s = warp; s < steps; s += kWarps) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
@@ -452,8 +487,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
             if (next >= kStages) next -= kStages;
             prefetch(s + (kStages - 1) * kWarps, next);
             const int t0 = lo + s * kStep;
-            step<D>(ring + slot * S::kStage, hi - t0, q, a, base, scale_limit, lane,
-                    p.scores ? p.scores + (rows + t0) * G : nullptr, G);
+            step<D>(ring + slot * S::kStage, hi - t0, q, a, lane, p.scores ? p.scores + rows * G + t0 : nullptr, p.max_seq, G);
             if (++slot == kStages) slot = 0;
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
@@ -484,17 +518,18 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float* row = results + (warp * kMaxGroup + 2 * j + c) * (D + S::kGroups);
-                const float even = f[c] * 16777216.f, odd = f[c] * 1048576.f;  // 2^24, and 2^20 for the high nibbles
+                const float even = f[c] * exp2f((float)(24 - a.k)), odd = even * 0.0625f;  // odd dims come from the high nibbles
 #pragma unroll
-                for (int i = 0; i < S::kGroups; ++i)
+                for (int i = 0; i < D / 32; ++i)
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        const int d = (i / S::kSpanGroups) * S::R::kSpan + (g >> 1) * (S::R::kSpan / 4) + 8 * (i % S::kSpanGroups) +
-                                      4 * (g & 1) + 2 * t;
-                        row[d] = a.o[i][t][c] * even;
-                        row[d + 1] = a.o[i][t][c + 2] * odd;
+                        const int d = 32 * i + 4 * g + 2 * t;
+                        *reinterpret_cast<float2*>(row + d) = make_float2(a.o[i][t][c] * even, a.o[i][t][c + 2] * odd);
                     }
-                if (g < S::kGroups) row[D + g] = a.lo[c] * f[c];
+                // each group's lanes hold the same
+                const int own = S::kSpanGroups == 4 ? g >> 1 : (g >> 1) & 1;
+                row[D + own] = a.lo[c] * f[c];
+                if (S::kSpans == 2) row[D + S::kSpanGroups + own] = a.lo[c + 2] * f[c];
             }
         }
         __syncthreads();
@@ -525,11 +560,14 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
     }
 }
 
-// The parts of (sequence, KV head) blockIdx.x that several CTAs worked on, query blockIdx.y.
-__global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const DecodeParams p, int dim) {
+// The parts of (sequence, KV head) blockIdx.x that several CTAs worked on, query blockIdx.y: every fourth part a warp.
+template <int D>
+__global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const DecodeParams p) {
+    constexpr int kPer = D / 32;  // dims of a lane
+    __shared__ float sums[kWarps][D], totals[kWarps];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int bh = blockIdx.x, b = bh / p.n_kv, h = blockIdx.y, G = p.group;
+    const int bh = blockIdx.x, b = bh / p.n_kv, h = blockIdx.y, G = p.group, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     int64_t before, all;
     count_tiles(p, b, before, all);
     const int n = tiles_of(visible(p, b));
@@ -539,18 +577,37 @@ __global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const DecodeParams 
     if (i0 == i1) return;  // one CTA had all of it
     // the first CTA's part is its last one, unless it begins with it
     const int64_t head = 2 * (int64_t)i0 + (share_start(i0, all, ctas) < t0);
-    auto part = [&](int i) { return i == i0 ? head : 2 * (int64_t)i; };
-    float m = -INFINITY, l = 0.f;
-    for (int i = i0; i <= i1; ++i) m = fmaxf(m, p.part_ml[part(i) * G + h].x);
-    for (int i = i0; i <= i1; ++i) {
-        const float2 x = p.part_ml[part(i) * G + h];
-        l += x.y * exp2f(x.x - m);
+    auto part = [&](int i) { return (i == i0 ? head : 2 * (int64_t)i) * G + h; };
+    float m = -INFINITY;
+    for (int i = i0 + lane; i <= i1; i += 32) m = fmaxf(m, p.part_ml[part(i)].x);
+#pragma unroll
+    for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
+    float o[kPer] = {}, l = 0.f;
+#pragma unroll 4
+    for (int i = i0 + warp; i <= i1; i += kWarps) {
+        const float2 x = p.part_ml[part(i)];
+        const float f = exp2f(x.x - m);
+        l += x.y * f;
+        const float* row = p.part_o + part(i) * D + lane * 2;
+#pragma unroll
+        for (int k = 0; k < kPer; k += 2) {
+            const float2 v = *reinterpret_cast<const float2*>(row + 32 * k);
+            o[k] = fmaf(v.x, f, o[k]), o[k + 1] = fmaf(v.y, f, o[k + 1]);
+        }
     }
+#pragma unroll
+    for (int k = 0; k < kPer; k += 2) *reinterpret_cast<float2*>(&sums[warp][32 * k + 2 * lane]) = make_float2(o[k], o[k + 1]);
+    if (lane == 0) totals[warp] = l;
+    __syncthreads();
+    l = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) l += totals[w];
     const int64_t row = (int64_t)bh * G + h;
-    for (int d = threadIdx.x; d < dim; d += kThreads) {
-        float o = 0.f;
-        for (int i = i0; i <= i1; ++i) o = fmaf(p.part_o[(part(i) * G + h) * dim + d], exp2f(p.part_ml[part(i) * G + h].x - m), o);
-        p.out[row * dim + d] = __float2bfloat16(o / l);
+    for (int d = threadIdx.x; d < D; d += kThreads) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) v += sums[w][d];
+        p.out[row * D + d] = __float2bfloat16(v / l);
     }
     if (threadIdx.x == 0 && p.lse) p.lse[row] = m * kLn2 + logf(l);
 }
@@ -562,9 +619,11 @@ __global__ void __launch_bounds__(kThreads) kv4_weights_kernel(const DecodeParam
     const int64_t b = blockIdx.z, bh = b * p.n_kv + blockIdx.y;
     const int len = visible(p, (int)b), t = blockIdx.x * kThreads + threadIdx.x;
     if (t >= len) return;
-    const float* x = p.scores + (bh * p.max_seq + t) * p.group;
+    const float* x = p.scores + bh * p.group * p.max_seq + t;
     float w = 0.f;
-    for (int h = 0; h < p.group; ++h) w += exp2f(x[h] - p.lse[bh * p.group + h] * kLog2e);
+#pragma unroll
+    for (int h = 0; h < kMaxGroup; ++h)
+        if (h < p.group) w += exp2f(x[h * p.max_seq] - p.lse[bh * p.group + h] * kLog2e);
     p.weights[bh * p.max_seq + t] += w;
 }
 
@@ -612,7 +671,7 @@ cudaError_t launch_kv4_decode(const Kv4Cache& c, const void* q, void* out, float
         if (e != cudaSuccess) return e;
         e = launch_chained(kv4_decode_kernel<D>, dim3(p.ctas), kThreads, Shape<D>::kSmem, stream, p);
         if (e == cudaSuccess && p.ctas > 1)
-            e = launch_chained(kv4_merge_kernel, dim3((unsigned)(batch * n_kv), p.group), kThreads, 0, stream, p, D);
+            e = launch_chained(kv4_merge_kernel<D>, dim3((unsigned)(batch * n_kv), p.group), kThreads, 0, stream, p);
         if (e == cudaSuccess && weights)
             e = launch_chained(kv4_weights_kernel, dim3((unsigned)((max_seq + kThreads - 1) / kThreads), n_kv, (unsigned)batch),
                                kThreads, 0, stream, p);
