@@ -2,10 +2,9 @@
 //
 // out = sum_t p_t v_t, p = softmax(scale * q . k_t), with k, v = lo + scale * code per group of 32 values.  Per group
 //     q . k = scale * sum(q * code) + lo * sum(q),        sum_t p_t v_t = sum_t p_t (scale_t code_t) + sum_t p_t lo_t.
-// A code in the low bits of a 16-bit half is the f16 subnormal code * 2^-24, which mma.sync multiplies exactly: one AND makes
-// a pair of operands, and the high nibble of a byte, 16 times as large, is met by a q (or a result row) that is 16 times
-// as small.  Keys need nothing else: the scale goes onto the 16 x 8 products.  Of V a product sums over tokens, so the
-// scale goes onto the codes (an f16 product, rounded to 11 bits).
+// A code in the low bits of a 16-bit half is the f16 subnormal code * 2^-24, which mma.sync multiplies exactly, and so is a
+// byte, two codes c0 + 16 c1: nothing is dequantised.  The scale of K goes onto the 16 x 8 products of a group, that of V, as
+// a product sums over tokens, onto the probabilities of a group's product.
 #include <algorithm>
 
 #include "cache_kernels.h"
@@ -18,17 +17,18 @@ namespace {
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kMaxGroup = 8;
 constexpr int kStep = 32;    // tokens of a warp's step
 constexpr int kTile = 64;    // tokens of a unit of work: the tiles of a launch are dealt to the CTAs in equal runs
-constexpr float kLazy = 4.f; // log2 of what a probability may exceed 1 by before the running maximum moves
+constexpr float kLazy = 6.f; // log2 of what a probability may exceed 1 by before the running maximum moves
 
 template <int D>
 struct Shape {
     using R = Kv4Row<D>;
     static constexpr int kGroups = R::kGroups, kSpanGroups = R::kSpanGroups, kSpans = D / R::kSpan;
     static constexpr int kRow = D / 2, kScaleRow = D / 8;
-    // Four lanes read rows 0, 2, 4 and 6 of V at a time: a pitch of 16 bytes more keeps them in different banks.
-    static constexpr int kVPitch = kRow + 16;
+    // A row of V lies group by group, 16 bytes each.  Eight rows are read at a time: a pitch of 16 bytes more keeps them in
+    // different banks.
+    static constexpr int kVPitch = kRow + 16, kVScalePitch = kScaleRow < 16 ? 16 : kScaleRow;
     static constexpr int kKBytes = kStep * kRow, kVBytes = kStep * kVPitch, kScaleBytes = kStep * kScaleRow;
-    static constexpr int kStage = kKBytes + kVBytes + 2 * kScaleBytes;
+    static constexpr int kStage = kKBytes + kVBytes + kScaleBytes + kStep * kVScalePitch;
     static constexpr int kStages = D == 256 ? 2 : 3;  // steps of a warp in shared memory
     static constexpr int kPerSm = D == 256 ? 2 : 3;   // CTAs resident on an SM
     static constexpr int kSmem = kWarps * kStages * kStage;
@@ -96,6 +96,13 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {  // 8x8 matrix of 16-bit values, a row's pair a lane
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -109,6 +116,11 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
     const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
+    const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t power_half2(int k) { return (uint32_t)(15 + k) * 0x04000400u; }  // 2^k twice, -15 < k < 16
 __device__ __forceinline__ float low_half(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)(w & 0xffffu))); }
 
 // Asynchronous copy of kBytes; `there` false writes zeros (and reads nothing).
@@ -118,7 +130,7 @@ __device__ __forceinline__ void copy_async(uint32_t to, const uint8_t* from, boo
     if constexpr (kBytes == 16)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
     else
-        asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(n) : "memory");
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(to), "l"(from), "r"(n), "n"(kBytes) : "memory");
 }
 
 // kWords neighbouring words of shared memory.
@@ -203,14 +215,17 @@ struct Queries {
 // What a warp has summed so far.  Lane (g, j) holds queries 2j and 2j + 1.
 template <int D>
 struct Sums {
-    float o[D / 32][2][4];       // [32 dims][0-1, 2-3 of a lane's four]: sum p scale code 2^(k - 24), {q 2j, 2j+1} x {even, odd dim}
-    float lo[4];                 // sum p * lo, row g = its group
+    float o[D / 32][2][4];       // [group][0-1, 2-3 of a lane's four dims]: sum p scale c 2^(k - 24), {q 2j, 2j+1} x {c0, c0 + 16 c1}
+    float lo[4];                 // sum p * lo: row 2i + 1 = group i, rows 8 and up the second span's
     float ref[2], top[2], l[2];  // p = 2^(score - ref); running maximum; sum of p (this lane's tokens)
-    int k;                       // scales are held times 2^k: the largest so far lies in [2^14, 2^15)
+    int k;                       // scales are held times 2^k: the largest so far lies in [1/2, 1), k is 15 at most
     uint32_t scale_limit;        // the largest f16 pattern for which k stands
 };
 constexpr float kBase = 15.f - kLazy;  // log2 of what p is held times: the largest reaches 2^15
 
+__device__ __forceinline__ void load_transposed(uint32_t (&r)[2], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at) : "memory");
+}
 __device__ __forceinline__ void load_transposed(uint32_t (&r)[4], uint32_t at) {  // four 8x8 matrices of 16-bit values
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -229,13 +244,14 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb) {
         const int r0 = tb * 16 + g, r1 = r0 + 8;
-        float m[4] = {0.f, 0.f, 0.f, 0.f};
+        float m[4];
 #pragma unroll
         for (int s = 0; s < S::kSpans; ++s) {  // sum(q) * lo: lane j brings its group
             const int at = (s * S::kSpanGroups + (j & (S::kSpanGroups - 1))) * 4;
             const uint32_t a0 = __byte_perm(*reinterpret_cast<const uint32_t*>(ks + r0 * S::kScaleRow + at), 0, 0x3232),
                            a1 = __byte_perm(*reinterpret_cast<const uint32_t*>(ks + r1 * S::kScaleRow + at), 0, 0x3232);
-            mma_f16(m, a0, a1, a0, a1, q.sums[s][0], q.sums[s][1]);
+            if (s == 0) mma_f16_first(m, a0, a1, a0, a1, q.sums[s][0], q.sums[s][1]);
+            else mma_f16(m, a0, a1, a0, a1, q.sums[s][0], q.sums[s][1]);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[tb][k] = m[k] * 3.814697265625e-06f;  // 64 * 2^-24
@@ -251,9 +267,9 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
 #pragma unroll
             for (int i = 0; i < S::kSpanGroups; ++i) {
                 const int gi = s * S::kSpanGroups + i;
-                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                mma_f16(c, w0[i] & 0x000f000fu, w1[i] & 0x000f000fu, w0[i] & 0x00f000f0u, w1[i] & 0x00f000f0u, q.even[gi][0],
-                        q.odd[gi][0]);
+                float c[4];
+                mma_f16_first(c, w0[i] & 0x000f000fu, w1[i] & 0x000f000fu, w0[i] & 0x00f000f0u, w1[i] & 0x00f000f0u, q.even[gi][0],
+                              q.odd[gi][0]);
                 const uint32_t h0 = w0[i] >> 8, h1 = w1[i] >> 8;
                 mma_f16(c, h0 & 0x000f000fu, h1 & 0x000f000fu, h0 & 0x00f000f0u, h1 & 0x00f000f0u, q.even[gi][1], q.odd[gi][1]);
                 const float f0 = low_half(s0[i]), f1 = low_half(s1[i]);
@@ -261,8 +277,6 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
                 x[tb][2] = fmaf(f1, c[2], x[tb][2]), x[tb][3] = fmaf(f1, c[3], x[tb][3]);
             }
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[tb][k] *= q.factor[k & 1];
     }
     if (valid < kStep) {
 #pragma unroll
@@ -280,30 +294,31 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
                 for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
                     for (int r = 0; r < 2; ++r)
-                        if (tb * 16 + 8 * r + g < valid) row[tb * 16 + 8 * r + g] = x[tb][2 * r + c];
+                        if (tb * 16 + 8 * r + g < valid) row[tb * 16 + 8 * r + g] = x[tb][2 * r + c] * q.factor[c];
             }
     }
     uint32_t big = 0;  // the largest scale of V: each lane looks at a token
 #pragma unroll
     for (int i = 0; i < S::kGroups; i += S::kSpanGroups) {
         uint32_t w[S::kSpanGroups];
-        load_words(w, vs + lane * S::kScaleRow + 4 * i);
+        load_words(w, vs + lane * S::kVScalePitch + 4 * i);
 #pragma unroll
-        for (int k = 0; k < S::kSpanGroups; ++k) big = max(big, w[k] & 0xffffu);
+        for (int k = 0; k < S::kSpanGroups; ++k) big = max_half2(big, w[k]);  // and the largest minimum, which is not looked at
     }
+    big &= 0xffffu;
     float top[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
         float m = fmaxf(fmaxf(x[0][c], x[0][c + 2]), fmaxf(x[1][c], x[1][c + 2]));
         m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 4));
         m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 8));
-        top[c] = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16));
+        top[c] = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16)) * q.factor[c];
     }
     if (__any_sync(kFullMask, top[0] > a.top[0] + kLazy || top[1] > a.top[1] + kLazy || big > a.scale_limit)) {
         big = __reduce_max_sync(kFullMask, big);
         float grow = 1.f;  // of the scales
         if (big > a.scale_limit) {
-            const int e = (int)(__float_as_uint(low_half(big)) >> 23) - 127, k = 14 - e;
+            const int e = (int)(__float_as_uint(low_half(big)) >> 23) - 127, k = min(-1 - e, 15);
             grow = exp2f((float)(k - a.k));
             a.k = k;
             a.scale_limit = (uint32_t)__half_as_ushort(__float2half_rn(exp2f((float)(e + 1)))) - 1;
@@ -334,53 +349,45 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
         float e[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            e[k] = fast_exp2(x[tb][k] - a.ref[k & 1]);
+            e[k] = fast_exp2(fmaf(x[tb][k], q.factor[k & 1], -a.ref[k & 1]));
             a.l[k & 1] += e[k];
         }
         // rounded to f16's 11 bits, an eighth of the result's own rounding to bf16
         prob[tb][0] = transposed(pack_half2(e[0], e[1]));
         prob[tb][1] = transposed(pack_half2(e[2], e[3]));
     }
-    const float up = __uint_as_float((uint32_t)(127 + a.k) << 23);
-    // V transposed: unit u (4 codes of one token) of a row's 16 bytes goes to the lanes g = u, tokens 2j and 2j + 1 in one
-    // register.  Lane g's units belong to one group of each span.
-    const int own = (S::kSpanGroups == 4 ? g >> 1 : (g >> 1) & 1) * 4;
+    const uint32_t up = power_half2(a.k);
+    // V and its scales come transposed: 16-bit unit g of a row (4 codes of a group, or a scale or minimum) to the lanes g, those
+    // of tokens 2j and 2j + 1 in one register.
     const uint32_t v_at = (uint32_t)__cvta_generic_to_shared(vc) + (lane & 15) * S::kVPitch + (lane >> 4) * 16;
+    const uint32_t s_at = (uint32_t)__cvta_generic_to_shared(vs) + (lane & 15) * S::kVScalePitch + (S::kSpans == 2 ? (lane >> 4) * 16 : 0);
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb) {
-        const uint8_t* at = vs + (tb * 16 + 2 * j) * S::kScaleRow + own;
+        uint32_t f[2 * S::kSpans];  // of tokens 0-7 and 8-15
+        load_transposed(f, s_at + tb * 16 * S::kVScalePitch);
+        if constexpr (S::kSpans == 2) mma_f16(a.lo, f[0], f[2], f[1], f[3], prob[tb][0], prob[tb][1]);
+        else mma_f16(a.lo, f[0], 0u, f[1], 0u, prob[tb][0], prob[tb][1]);
 #pragma unroll
-        for (int s = 0; s < S::kSpans; ++s) {
-            uint32_t f[4];  // {scale, lo} of tokens 2j, 2j + 1, 2j + 8, 2j + 9
+        for (int k = 0; k < 2 * S::kSpans; ++k) f[k] = mul_half2(f[k], up);
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                f[k] = *reinterpret_cast<const uint32_t*>(at + s * 4 * S::kSpanGroups + ((k & 1) + 4 * (k & 2)) * S::kScaleRow);
-            // sum p * lo: row g of the product is lane g's group, rows 8 and up of the second span
-            const uint32_t lo0 = __byte_perm(f[0], f[1], 0x7632), lo1 = __byte_perm(f[2], f[3], 0x7632);
-            if (s == 0) mma_f16(a.lo, lo0, 0u, lo1, 0u, prob[tb][0], prob[tb][1]);
-            else mma_f16(a.lo, 0u, lo0, 0u, lo1, prob[tb][0], prob[tb][1]);
-            const uint32_t s0 = pack_half2(low_half(f[0]) * up, low_half(f[1]) * up),
-                           s1 = pack_half2(low_half(f[2]) * up, low_half(f[3]) * up);
+        for (int gi = 0; gi < S::kGroups; gi += 2) {
+            uint32_t w[4];  // group gi, tokens 0-7 and 8-15; group gi + 1
+            load_transposed(w, v_at + tb * 16 * S::kVPitch + gi * 16);
 #pragma unroll
-            for (int i = 0; i < S::R::kSpan / 32; i += 2) {
-                const int gi = s * (S::R::kSpan / 32) + i;
-                uint32_t w[4];  // 32 dims, tokens 0-7 and 8-15; the next 32
-                load_transposed(w, v_at + tb * 16 * S::kVPitch + gi * 16);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t u0 = w[2 * c], u1 = w[2 * c + 1];
-                    mma_f16(a.o[gi + c][0], mul_half2(u0 & 0x000f000fu, s0), mul_half2(u0 & 0x00f000f0u, s0),
-                            mul_half2(u1 & 0x000f000fu, s1), mul_half2(u1 & 0x00f000f0u, s1), prob[tb][0], prob[tb][1]);
-                    u0 >>= 8, u1 >>= 8;
-                    mma_f16(a.o[gi + c][1], mul_half2(u0 & 0x000f000fu, s0), mul_half2(u0 & 0x00f000f0u, s0),
-                            mul_half2(u1 & 0x000f000fu, s1), mul_half2(u1 & 0x00f000f0u, s1), prob[tb][0], prob[tb][1]);
-                }
+            for (int c = 0; c < 2; ++c) {
+                const int s = (gi + c) / S::kSpanGroups, from = 8 * ((gi + c) % S::kSpanGroups) + j;
+                const uint32_t b0 = mul_half2(prob[tb][0], __shfl_sync(kFullMask, f[2 * s], from)),
+                               b1 = mul_half2(prob[tb][1], __shfl_sync(kFullMask, f[2 * s + 1], from));
+                uint32_t u0 = w[2 * c], u1 = w[2 * c + 1];
+                mma_f16(a.o[gi + c][0], u0 & 0x000f000fu, u0 & 0x00ff00ffu, u1 & 0x000f000fu, u1 & 0x00ff00ffu, b0, b1);
+                u0 = __byte_perm(u0, 0, 0x4341), u1 = __byte_perm(u1, 0, 0x4341);
+                mma_f16(a.o[gi + c][1], u0 & 0x000f000fu, u0, u1 & 0x000f000fu, u1, b0, b1);
             }
         }
     }
 }
 
-// A lane's places in the planes: the step's bytes are contiguous, 16 neighbouring ones a lane and copy.
+// A lane's places in the planes: the step's bytes are contiguous, neighbouring pieces a lane and copy.
 struct LanePlanes {
     const uint8_t *k, *v, *ks, *vs;
 };
@@ -389,30 +396,36 @@ struct LanePlanes {
 template <int D>
 __device__ __forceinline__ void fetch(uint32_t to, const LanePlanes& from, int64_t token, int valid, int lane) {
     using S = Shape<D>;
-    constexpr int kChunks = S::kRow / 16;  // of a row's codes
-    constexpr int kRows = 32 / kChunks;    // that a copy of the warp covers
+    constexpr int kChunks = S::kRow / 16, kWords = S::kRow / 4;  // of a row's codes
     constexpr int kPiece = S::kScaleRow < 16 ? S::kScaleRow : 16, kPieces = S::kScaleRow / kPiece;
-    const int r = lane / kChunks, c = lane % kChunks, r_scale = lane / kPieces;
+    const int r = lane / kChunks, c = lane % kChunks, rv = lane / kWords, o = lane % kWords, rs = lane / kPieces;
     // at D = 256 odd rows have their spans swapped
     const uint32_t k_to = to + r * S::kRow + (S::kSpans == 2 ? c ^ ((r & 1) << 2) : c) * 16;
-    const uint32_t v_to = to + S::kKBytes + r * S::kVPitch + c * 16;
-    const uint32_t s_to = to + S::kKBytes + S::kVBytes + lane * kPiece;
+    // V word by word: octet o of a row is a group's word (o % kSpanOctets) / kSpanGroups
+    const uint32_t v_to = to + S::kKBytes + rv * S::kVPitch + S::R::group_of_octet(o) * 16 + (o % S::R::kSpanOctets) / S::kSpanGroups * 4;
+    const uint32_t ks_to = to + S::kKBytes + S::kVBytes + lane * kPiece;
+    const uint32_t vs_to = to + S::kKBytes + S::kVBytes + S::kScaleBytes + rs * S::kVScalePitch + lane % kPieces * kPiece;
     const uint8_t *k = from.k + token * S::kRow, *v = from.v + token * S::kRow;
     const uint8_t *ks = from.ks + token * S::kScaleRow, *vs = from.vs + token * S::kScaleRow;
-    static_assert(kRows % 2 == 0, "a row's parity is the same in all copies of a lane");
+    static_assert((32 / kChunks) % 2 == 0, "a row's parity is the same in all copies of a lane");
 #pragma unroll
     for (int n = 0; n < kChunks; ++n) {
+        constexpr int kRows = 32 / kChunks;
         const bool there = valid >= kStep || r + n * kRows < valid;
-        const int64_t at = there ? n * 512 : 0;
-        copy_async<16>(k_to + n * kRows * S::kRow, there ? k + at : from.k - lane * 16, there);
-        copy_async<16>(v_to + n * kRows * S::kVPitch, there ? v + at : from.v - lane * 16, there);
+        copy_async<16>(k_to + n * kRows * S::kRow, there ? k + n * 512 : from.k - lane * 16, there);
+    }
+#pragma unroll
+    for (int n = 0; n < kWords; ++n) {
+        constexpr int kRows = 32 / kWords;
+        const bool there = valid >= kStep || rv + n * kRows < valid;
+        copy_async<4>(v_to + n * kRows * S::kVPitch, there ? v + n * 128 : from.v - lane * 4, there);
     }
 #pragma unroll
     for (int n = 0; n < kPieces; ++n) {
-        const bool there = valid >= kStep || r_scale + n * (32 / kPieces) < valid;
-        const int64_t at = there ? n * 32 * kPiece : 0;
-        copy_async<kPiece>(s_to + n * 32 * kPiece, there ? ks + at : from.ks - lane * kPiece, there);
-        copy_async<kPiece>(s_to + S::kScaleBytes + n * 32 * kPiece, there ? vs + at : from.vs - lane * kPiece, there);
+        constexpr int kRows = 32 / kPieces;
+        const bool there = valid >= kStep || rs + n * kRows < valid;
+        copy_async<kPiece>(ks_to + n * 32 * kPiece, there ? ks + n * 32 * kPiece : from.ks - lane * kPiece, there);
+        copy_async<kPiece>(vs_to + n * kRows * S::kVScalePitch, there ? vs + n * 32 * kPiece : from.vs - lane * kPiece, there);
     }
 }
 
@@ -457,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
     uint8_t* ring = smem + warp * kStages * S::kStage;
     const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
     constexpr int kPiece = S::kScaleRow < 16 ? S::kScaleRow : 16;
-    const LanePlanes planes{p.k_codes + lane * 16, p.v_codes + lane * 16, p.k_scales + lane * kPiece, p.v_scales + lane * kPiece};
+    const LanePlanes planes{p.k_codes + lane * 16, p.v_codes + lane * 4, p.k_scales + lane * kPiece, p.v_scales + lane * kPiece};
     for (bool head = true; at < end; head = false) {
         const int len = visible(p, b), n = tiles_of(len);
         const int h = (int)((at - first) / n), tile = (int)((at - first) % n);
@@ -518,18 +531,19 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 float* row = results + (warp * kMaxGroup + 2 * j + c) * (D + S::kGroups);
-                const float even = f[c] * exp2f((float)(24 - a.k)), odd = even * 0.0625f;  // odd dims come from the high nibbles
+                const float even = f[c] * exp2f((float)(24 - a.k)), odd = even * 0.0625f;
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i)
+                for (int i = 0; i < S::kGroups; ++i)
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
-                        const int d = 32 * i + 4 * g + 2 * t;
-                        *reinterpret_cast<float2*>(row + d) = make_float2(a.o[i][t][c] * even, a.o[i][t][c + 2] * odd);
+                        const int d = (i / S::kSpanGroups) * S::R::kSpan + (g >> 1) * (S::R::kSpan / 4) + 8 * (i % S::kSpanGroups) +
+                                      4 * (g & 1) + 2 * t;
+                        *reinterpret_cast<float2*>(row + d) = make_float2(a.o[i][t][c] * even, (a.o[i][t][c + 2] - a.o[i][t][c]) * odd);
                     }
-                // each group's lanes hold the same
-                const int own = S::kSpanGroups == 4 ? g >> 1 : (g >> 1) & 1;
-                row[D + own] = a.lo[c] * f[c];
-                if (S::kSpans == 2) row[D + S::kSpanGroups + own] = a.lo[c + 2] * f[c];
+                if ((g & 1) && (g >> 1) < S::kSpanGroups) {
+                    row[D + (g >> 1)] = a.lo[c] * f[c];
+                    if (S::kSpans == 2) row[D + S::kSpanGroups + (g >> 1)] = a.lo[c + 2] * f[c];
+                }
             }
         }
         __syncthreads();

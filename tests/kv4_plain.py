@@ -79,10 +79,11 @@ def decode(q, cache, lens, scale=None):
         size = torch.einsum("hgd,htd->hgt", qb.abs(), k.abs() + 15 * cache.k_scales[b, :, :n, :, 0].double()[..., groups(D).to(q.device)]) * scale
         ds = size.amax(-1) * (2 * D + 8) * U_F32 + 16 * U_F32 * (1 + s.abs().amax(-1))
         lse_tol[b] = (ds + 16 * U_F32 * (1 + m.abs())).reshape(Hq)
-        # p is rounded to f16, and once more with its token's scale (or, below 2^-29 of the largest, to a step of 2^-39);
-        # the result to bf16
+        # p is rounded to f16, and its product with a token's scale once more; the result to bf16.  p is held times 2^9 and the
+        # scale so that the largest is in [1/2, 1): f16's last place, 2^-24, is 2^-33 of p's unit and of twice the largest
+        # scale's, and half of it is lost of each.
         near = torch.einsum("hgt,htd->hgd", p, v.abs() + step)
-        near = near * (2.1 * U_F16) + near * (2 * ds)[..., None] + n * 2.0 ** -39 * (v.abs().max() + step.max().clamp(min=15))
+        near = near * (2.1 * U_F16) + near * (2 * ds)[..., None] + n * 2.0 ** -33 * (v.abs().max() + step.max())
         out_tol[b] = (near * (1 + U_BF16)).reshape(Hq, D) + U_BF16 * out[b].abs() + 2.0 ** -40
         w_tol[b, :, :n] = (p * (2 * ds + 64 * U_F32 * (1 + m.abs()))[..., None]).sum(1)
     return out, lse, w, out_tol, lse_tol, w_tol
