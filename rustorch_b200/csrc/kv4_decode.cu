@@ -31,10 +31,12 @@ struct Shape {
     static constexpr int kStage = kKBytes + kVBytes + kScaleBytes + kStep * kVScalePitch;
     static constexpr int kStages = D == 256 ? 2 : 3;  // steps of a warp in shared memory
     static constexpr int kPerSm = D == 256 ? 2 : 3;   // CTAs resident on an SM
-    static constexpr int kSmem = kWarps * kStages * kStage;
+    static constexpr int kRing = kWarps * kStages * kStage;
+    static constexpr int kSmem = kRing + (kGroups + 1) * 512;  // and the queries as operands
     // The warps' results lie over the ring once it has run dry.
-    static constexpr int kMerge = kWarps * (kMaxGroup * (D + kGroups) + 2 * kMaxGroup) * 4;
-    static_assert(kMerge <= kSmem && kStage % 16 == 0, "the merge fits the ring");
+    static constexpr int kResult = D + 8;  // of a query: its sums, and those of its groups' minima
+    static constexpr int kMerge = kWarps * kMaxGroup * (kResult * 4 + 8) + kMaxGroup * 8;
+    static_assert(kMerge <= kRing && kStage % 16 == 0, "the merge fits the ring");
 };
 
 struct DecodeParams {
@@ -96,6 +98,11 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(b));
+}
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                               uint32_t b1) {
     asm volatile(
@@ -151,7 +158,7 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[kWords], const uint8_t*
 template <int D>
 struct Queries {
     uint32_t even[Shape<D>::kGroups][2], odd[Shape<D>::kGroups][2];  // pairs (0,4), (2,6) and (1,5)/16, (3,7)/16 of an octet
-    uint32_t sums[Shape<D>::kSpans][2];  // a group's sum / 64 in three f16 parts (and 0): 33 bits
+    uint32_t sums[Shape<D>::kSpans];     // lane j's group of a span: its sum / 64 in two f16 parts, 22 bits
     float factor[2];                     // scale_log2 * 2^24 / the power of two, of queries 2j and 2j + 1
 
     __device__ __forceinline__ void load(const DecodeParams& p, int64_t bh, int lane) {
@@ -200,8 +207,7 @@ struct Queries {
             float t = 0.f;  // lane j's group of the span
 #pragma unroll
             for (int i = 0; i < S::kSpanGroups; ++i) t = j == i ? total[s * S::kSpanGroups + i] * 0.015625f : t;
-            const float a = __half2float(__float2half_rn(t)), b = __half2float(__float2half_rn(t - a));
-            sums[s][0] = pack_half2(a, b), sums[s][1] = pack_half2(t - a - b, 0.f);
+            sums[s] = pack_half2(t, t - __half2float(__float2half_rn(t)));
         }
         // NaN and infinite queries: the row is NaN whatever the codes are
         float f = nan || top == INFINITY ? __uint_as_float(0x7fffffffu) : p.scale_log2 * exp2f((float)(24 - e));
@@ -216,16 +222,13 @@ struct Queries {
 template <int D>
 struct Sums {
     float o[D / 32][2][4];       // [group][0-1, 2-3 of a lane's four dims]: sum p scale c 2^(k - 24), {q 2j, 2j+1} x {c0, c0 + 16 c1}
-    float lo[4];                 // sum p * lo: row 2i + 1 = group i, rows 8 and up the second span's
+    float lo[4], lo2[4];         // sum p * lo: row 2i + 1 = group i; see `step` for which of the rows count
     float ref[2], top[2], l[2];  // p = 2^(score - ref); running maximum; sum of p (this lane's tokens)
     int k;                       // scales are held times 2^k: the largest so far lies in [1/2, 1), k is 15 at most
     uint32_t scale_limit;        // the largest f16 pattern for which k stands
 };
 constexpr float kBase = 15.f - kLazy;  // log2 of what p is held times: the largest reaches 2^15
 
-__device__ __forceinline__ void load_transposed(uint32_t (&r)[2], uint32_t at) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];" : "=r"(r[0]), "=r"(r[1]) : "r"(at) : "memory");
-}
 __device__ __forceinline__ void load_transposed(uint32_t (&r)[4], uint32_t at) {  // four 8x8 matrices of 16-bit values
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -244,14 +247,13 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb) {
         const int r0 = tb * 16 + g, r1 = r0 + 8;
-        float m[4];
+        float m[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = 0; s < S::kSpans; ++s) {  // sum(q) * lo: lane j brings its group
             const int at = (s * S::kSpanGroups + (j & (S::kSpanGroups - 1))) * 4;
             const uint32_t a0 = __byte_perm(*reinterpret_cast<const uint32_t*>(ks + r0 * S::kScaleRow + at), 0, 0x3232),
                            a1 = __byte_perm(*reinterpret_cast<const uint32_t*>(ks + r1 * S::kScaleRow + at), 0, 0x3232);
-            if (s == 0) mma_f16_first(m, a0, a1, a0, a1, q.sums[s][0], q.sums[s][1]);
-            else mma_f16(m, a0, a1, a0, a1, q.sums[s][0], q.sums[s][1]);
+            mma_f16_k8(m, a0, a1, q.sums[s]);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[tb][k] = m[k] * 3.814697265625e-06f;  // 64 * 2^-24
@@ -334,7 +336,7 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
             a.l[c] *= alpha[c];
         }
 #pragma unroll
-        for (int k = 0; k < 4; ++k) a.lo[k] *= alpha[k & 1];
+        for (int k = 0; k < 4; ++k) a.lo[k] *= alpha[k & 1], a.lo2[k] *= alpha[k & 1];
         alpha[0] *= grow, alpha[1] *= grow;
 #pragma unroll
         for (int i = 0; i < S::kGroups; ++i)
@@ -360,15 +362,31 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
     // V and its scales come transposed: 16-bit unit g of a row (4 codes of a group, or a scale or minimum) to the lanes g, those
     // of tokens 2j and 2j + 1 in one register.
     const uint32_t v_at = (uint32_t)__cvta_generic_to_shared(vc) + (lane & 15) * S::kVPitch + (lane >> 4) * 16;
-    const uint32_t s_at = (uint32_t)__cvta_generic_to_shared(vs) + (lane & 15) * S::kVScalePitch + (S::kSpans == 2 ? (lane >> 4) * 16 : 0);
+    // The scales of D = 256 are four matrices for 16 tokens, spans as rows 0-7 and 8-15 of one operand.  Else they are one
+    // for 8 tokens: those of 32 tokens make an operand whose rows 0-7 count in the product with the tokens 0-7 and 16-23,
+    // and rows 8-15 in that with the others.
+    const uint32_t s_at = (uint32_t)__cvta_generic_to_shared(vs) +
+                          (S::kSpans == 2 ? ((lane & 7) + (lane >> 4) * 8) * S::kVScalePitch + (lane >> 3 & 1) * 16 : lane * S::kVScalePitch);
+    uint32_t f[2][2][S::kSpans];  // [16 tokens][8 tokens][span]
+    if constexpr (S::kSpans == 2) {
+#pragma unroll
+        for (int tb = 0; tb < 2; ++tb) {
+            uint32_t w[4];
+            load_transposed(w, s_at + tb * 16 * S::kVScalePitch);
+            mma_f16(a.lo, w[0], w[1], w[2], w[3], prob[tb][0], prob[tb][1]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[tb][k / 2][k % 2] = mul_half2(w[k], up);
+        }
+    } else {
+        uint32_t w[4];
+        load_transposed(w, s_at);
+        mma_f16(a.lo, w[0], w[1], w[2], w[3], prob[0][0], prob[1][0]);
+        mma_f16(a.lo2, w[0], w[1], w[2], w[3], prob[0][1], prob[1][1]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k / 2][k % 2][0] = mul_half2(w[k], up);
+    }
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb) {
-        uint32_t f[2 * S::kSpans];  // of tokens 0-7 and 8-15
-        load_transposed(f, s_at + tb * 16 * S::kVScalePitch);
-        if constexpr (S::kSpans == 2) mma_f16(a.lo, f[0], f[2], f[1], f[3], prob[tb][0], prob[tb][1]);
-        else mma_f16(a.lo, f[0], 0u, f[1], 0u, prob[tb][0], prob[tb][1]);
-#pragma unroll
-        for (int k = 0; k < 2 * S::kSpans; ++k) f[k] = mul_half2(f[k], up);
 #pragma unroll
         for (int gi = 0; gi < S::kGroups; gi += 2) {
             uint32_t w[4];  // group gi, tokens 0-7 and 8-15; group gi + 1
@@ -376,8 +394,8 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int s = (gi + c) / S::kSpanGroups, from = 8 * ((gi + c) % S::kSpanGroups) + j;
-                const uint32_t b0 = mul_half2(prob[tb][0], __shfl_sync(kFullMask, f[2 * s], from)),
-                               b1 = mul_half2(prob[tb][1], __shfl_sync(kFullMask, f[2 * s + 1], from));
+                const uint32_t b0 = mul_half2(prob[tb][0], __shfl_sync(kFullMask, f[tb][0][s], from)),
+                               b1 = mul_half2(prob[tb][1], __shfl_sync(kFullMask, f[tb][1][s], from));
                 uint32_t u0 = w[2 * c], u1 = w[2 * c + 1];
                 mma_f16(a.o[gi + c][0], u0 & 0x000f000fu, u0 & 0x00ff00ffu, u1 & 0x000f000fu, u1 & 0x00ff00ffu, b0, b1);
                 u0 = __byte_perm(u0, 0, 0x4341), u1 = __byte_perm(u1, 0, 0x4341);
@@ -488,8 +506,26 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
         };
 #pragma unroll
         for (int i = 0; i < kStages - 1; ++i) prefetch(warp + i * kWarps, i);
+        // one warp lays the queries out for all
         Queries<D> q;
-        q.load(p, bh, lane);
+        uint4* shared_q = reinterpret_cast<uint4*>(smem + S::kRing) + lane;
+        if (warp == 0) {
+            q.load(p, bh, lane);
+#pragma unroll
+            for (int i = 0; i < S::kGroups; ++i)
+                shared_q[i * 32] = make_uint4(q.even[i][0], q.odd[i][0], q.even[i][1], q.odd[i][1]);
+            shared_q[S::kGroups * 32] = make_uint4(q.sums[0], q.sums[S::kSpans - 1], __float_as_uint(q.factor[0]), __float_as_uint(q.factor[1]));
+        }
+        __syncthreads();
+        if (warp != 0) {
+#pragma unroll
+            for (int i = 0; i < S::kGroups; ++i) {
+                const uint4 x = shared_q[i * 32];
+                q.even[i][0] = x.x, q.odd[i][0] = x.y, q.even[i][1] = x.z, q.odd[i][1] = x.w;
+            }
+            const uint4 x = shared_q[S::kGroups * 32];
+            q.sums[0] = x.x, q.sums[S::kSpans - 1] = x.y, q.factor[0] = __uint_as_float(x.z), q.factor[1] = __uint_as_float(x.w);
+        }
         Sums<D> a = {};
         a.top[0] = a.top[1] = -INFINITY;
         int slot = 0;
@@ -509,63 +545,76 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
         for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) a.l[c] += __shfl_xor_sync(kFullMask, a.l[c], off);
-        float* results = reinterpret_cast<float*>(smem);             // [warp][query][D + groups]
-        float2* ml = reinterpret_cast<float2*>(results + kWarps * kMaxGroup * (D + S::kGroups));  // [warp][query]
+        float* results = reinterpret_cast<float*>(smem);  // [warp][query][kResult]
+        float2* ml = reinterpret_cast<float2*>(results + kWarps * kMaxGroup * S::kResult);  // [warp][query]
+        float2* total = ml + kWarps * kMaxGroup;                                           // [query]
+        const int g = lane / 4, j = lane % 4;
         __syncthreads();
-        if (lane < 4) {
-            ml[warp * kMaxGroup + 2 * lane] = make_float2(a.top[0] == -INFINITY && a.l[0] == 0.f ? -INFINITY : a.ref[0], a.l[0]);
-            ml[warp * kMaxGroup + 2 * lane + 1] = make_float2(a.top[1] == -INFINITY && a.l[1] == 0.f ? -INFINITY : a.ref[1], a.l[1]);
+        if (g == 0) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                ml[warp * kMaxGroup + 2 * j + c] = make_float2(a.top[c] == -INFINITY && a.l[c] == 0.f ? -INFINITY : a.ref[c], a.l[c]);
         }
         __syncthreads();
-        {
-            const int g = lane / 4, j = lane % 4;
-            float f[2];
+        if (tid < kMaxGroup) {
+            float m = -INFINITY, l = 0.f;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float m = -INFINITY;
+            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * kMaxGroup + tid].x);
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * kMaxGroup + 2 * j + c].x);
-                const float mine = ml[warp * kMaxGroup + 2 * j + c].x;
-                f[c] = mine == -INFINITY ? 0.f : exp2f(mine - m);
+            for (int w = 0; w < kWarps; ++w) {
+                const float2 x = ml[w * kMaxGroup + tid];
+                if (x.x != -INFINITY) l += x.y * exp2f(x.x - m);
             }
+            total[tid] = make_float2(m, l);
+        }
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float* row = results + (warp * kMaxGroup + 2 * j + c) * (D + S::kGroups);
-                const float even = f[c] * exp2f((float)(24 - a.k)), odd = even * 0.0625f;
+        for (int c = 0; c < 2; ++c) {
+            float m = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < S::kGroups; ++i)
+            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * kMaxGroup + 2 * j + c].x);
+            const float mine = ml[warp * kMaxGroup + 2 * j + c].x, f = mine == -INFINITY ? 0.f : exp2f(mine - m);
+            float* row = results + (warp * kMaxGroup + 2 * j + c) * S::kResult;
+            const float even = f * exp2f((float)(24 - a.k)), odd = even * 0.0625f;
+            if (2 * j + c < G) {
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const int d = (i / S::kSpanGroups) * S::R::kSpan + (g >> 1) * (S::R::kSpan / 4) + 8 * (i % S::kSpanGroups) +
-                                      4 * (g & 1) + 2 * t;
-                        *reinterpret_cast<float2*>(row + d) = make_float2(a.o[i][t][c] * even, (a.o[i][t][c + 2] - a.o[i][t][c]) * odd);
-                    }
+                for (int i = 0; i < S::kGroups; ++i) {
+                    const int d = (i / S::kSpanGroups) * S::R::kSpan + (g >> 1) * (S::R::kSpan / 4) + 8 * (i % S::kSpanGroups) + 4 * (g & 1);
+                    *reinterpret_cast<float4*>(row + d) =
+                        make_float4(a.o[i][0][c] * even, (a.o[i][0][c + 2] - a.o[i][0][c]) * odd, a.o[i][1][c] * even,
+                                    (a.o[i][1][c + 2] - a.o[i][1][c]) * odd);
+                }
                 if ((g & 1) && (g >> 1) < S::kSpanGroups) {
-                    row[D + (g >> 1)] = a.lo[c] * f[c];
-                    if (S::kSpans == 2) row[D + S::kSpanGroups + (g >> 1)] = a.lo[c + 2] * f[c];
+                    if (S::kSpans == 2) {
+                        row[D + (g >> 1)] = a.lo[c] * f;
+                        row[D + S::kSpanGroups + (g >> 1)] = a.lo[c + 2] * f;
+                    } else {
+                        row[D + (g >> 1)] = (a.lo[c] + a.lo2[c + 2]) * f;
+                    }
                 }
             }
         }
         __syncthreads();
         const int64_t part = 2 * (int64_t)blockIdx.x + !head;
-        for (int i = tid; i < G * D; i += kThreads) {
-            const int h = i / D, d = i % D;
-            float m = -INFINITY, l = 0.f, o = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * kMaxGroup + h].x);
+        for (int i = tid; i < G * (D / 4); i += kThreads) {
+            const int q_at = i / (D / 4), d = i % (D / 4) * 4;
+            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const float2 x = ml[w * kMaxGroup + h];
-                const float* row = results + (w * kMaxGroup + h) * (D + S::kGroups);
-                l += x.x == -INFINITY ? 0.f : x.y * exp2f(x.x - m);
-                o += row[d] + row[D + S::R::group_of_octet(d / 8)];
+                const float* row = results + (w * kMaxGroup + q_at) * S::kResult;
+                const float4 x = *reinterpret_cast<const float4*>(row + d);
+                const float y = row[D + S::R::group_of_octet(d / 8)];
+                o.x += x.x + y, o.y += x.y + y, o.z += x.z + y, o.w += x.w + y;
             }
+            const float2 t = total[q_at];
             if (whole) {
-                p.out[(bh * G + h) * D + d] = __float2bfloat16(hi > lo ? o / l : 0.f);
-                if (d == 0 && p.lse) p.lse[bh * G + h] = hi > lo ? m * kLn2 + logf(l) : -INFINITY;
+                const float inv = hi > lo ? 1.f / t.y : 0.f;
+                const uint2 packed = make_uint2(float2_to_bf16x2(hi > lo ? o.x * inv : 0.f, hi > lo ? o.y * inv : 0.f),
+                                                float2_to_bf16x2(hi > lo ? o.z * inv : 0.f, hi > lo ? o.w * inv : 0.f));
+                *reinterpret_cast<uint2*>(p.out + (bh * G + q_at) * D + d) = packed;
+                if (d == 0 && p.lse) p.lse[bh * G + q_at] = hi > lo ? t.x * kLn2 + logf(t.y) : -INFINITY;
             } else {
-                p.part_o[(part * G + h) * D + d] = o;
-                if (d == 0) p.part_ml[part * G + h] = make_float2(m, l);
+                *reinterpret_cast<float4*>(p.part_o + (part * G + q_at) * D + d) = o;
+                if (d == 0) p.part_ml[part * G + q_at] = t;
             }
         }
         __syncthreads();
