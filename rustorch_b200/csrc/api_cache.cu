@@ -110,7 +110,7 @@ int rt_kv4_decode(const void* q, const void* k_codes, const void* k_scales, cons
     if (n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads != 0) return RT_ERR_HEAD_COUNT;
     if (const int rc = check_shape(batch, n_kv_heads, head_dim, max_seq)) return rc;
     if (max_seq == 0 || (!kv_lens && (kv_len_uniform < 0 || kv_len_uniform > max_seq))) return RT_ERR_BAD_LENGTH;
-    if (n_heads / n_kv_heads > 8) return RT_ERR_UNSUPPORTED;
+    if (n_heads / n_kv_heads > 8 || batch * n_heads > 0x7fffffff) return RT_ERR_UNSUPPORTED;
     if (batch == 0) return RT_OK;
     const rt::Kv4Cache c{k_codes, k_scales, v_codes, v_scales};
     if (!q || !out) return RT_ERR_NULL_POINTER;

@@ -15,8 +15,7 @@ namespace rt {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kMaxGroup = 8;
-constexpr int kStep = 32;    // tokens of a warp's step
-constexpr int kTile = 64;    // tokens of a unit of work: the tiles of a launch are dealt to the CTAs in equal runs
+constexpr int kStep = 32;    // tokens of a warp's step; the steps of a launch are dealt to its warps in equal runs
 constexpr float kLazy = 6.f; // log2 of what a probability may exceed 1 by before the running maximum moves
 
 template <int D>
@@ -31,12 +30,8 @@ struct Shape {
     static constexpr int kStage = kKBytes + kVBytes + kScaleBytes + kStep * kVScalePitch;
     static constexpr int kStages = D == 256 ? 2 : 3;  // steps of a warp in shared memory
     static constexpr int kPerSm = D == 256 ? 2 : 3;   // CTAs resident on an SM
-    static constexpr int kRing = kWarps * kStages * kStage;
-    static constexpr int kSmem = kRing + (kGroups + 1) * 512;  // and the queries as operands
-    // The warps' results lie over the ring once it has run dry.
-    static constexpr int kResult = D + 8;  // of a query: its sums, and those of its groups' minima
-    static constexpr int kMerge = kWarps * kMaxGroup * (kResult * 4 + 8) + kMaxGroup * 8;
-    static_assert(kMerge <= kRing && kStage % 16 == 0, "the merge fits the ring");
+    static constexpr int kSmem = kWarps * kStages * kStage;
+    static_assert(kStage % 16 == 0, "copies are of 16 bytes");
 };
 
 struct DecodeParams {
@@ -46,66 +41,56 @@ struct DecodeParams {
     float* lse;
     float* weights;
     float* scores;   // [B * Hq, max_seq] scaled scores (log2), where weights are asked for
-    float* part_o;   // [2 * CTAs][group][D]
-    float2* part_ml; // [2 * CTAs][group]: the reference that the part's sums are relative to (log2), the sum of its weights
+    float* part_o;   // [2 * workers][group][D]
+    float2* part_ml; // [2 * workers][group]: the reference that the part's sums are relative to (log2), the sum of its weights
+    int2* spans;     // [B * Hkv]: the first part of each and the worker that has the last one; x = -1 where there are no parts
     int64_t max_seq;
     const int32_t* kv_lens;
-    int kv_len, batch, n_kv, group, ctas;
+    int kv_len, batch, n_kv, group, workers;  // workers: warps that take a run of steps
     float scale_log2;
 };
 
 __device__ __forceinline__ int visible(const DecodeParams& p, int b) {
     return max(0, (int)min(p.kv_lens ? (int64_t)p.kv_lens[b] : (int64_t)p.kv_len, p.max_seq));
 }
-// A sequence without tokens has one tile too: somebody has to write its zeros.
-__device__ __forceinline__ int tiles_of(int len) { return max(1, (len + kTile - 1) / kTile); }
+// A sequence without tokens has one step too: somebody has to write its zeros.
+__device__ __forceinline__ int steps_of(int len) { return max(1, (len + kStep - 1) / kStep); }
 
-// Tiles are numbered sequence by sequence, KV head by KV head; CTA i takes [i * all / ctas, (i + 1) * all / ctas),
-// with no more CTAs than tiles, so that every one has a part.
-__device__ __forceinline__ int64_t share_start(int64_t i, int64_t all, int ctas) { return i * all / ctas; }
-__device__ __forceinline__ int share_of(int64_t tile, int64_t all, int ctas) { return (int)(((tile + 1) * ctas - 1) / all); }
+// Steps are numbered sequence by sequence, KV head by KV head; worker i takes [i * all / workers, (i + 1) * all / workers),
+// with no more workers than steps, so that every one has a part.
+__device__ __forceinline__ int64_t share_start(int64_t i, int64_t all, int workers) { return i * all / workers; }
 
-// Sum of the tiles of sequences [0, n) and of all, for all threads of the CTA.
-__device__ __forceinline__ void count_tiles(const DecodeParams& p, int n, int64_t& before, int64_t& all) {
-    if (!p.kv_lens) {
-        const int64_t t = tiles_of(visible(p, 0));
-        before = t * n * p.n_kv, all = t * p.batch * p.n_kv;
-        return;
-    }
-    __shared__ int64_t sums[kWarps][2];
-    int64_t x = 0, y = 0;
-    for (int b = threadIdx.x; b < p.batch; b += kThreads) {
-        const int t = tiles_of(visible(p, b));
-        x += b < n ? t : 0, y += t;
-    }
+// Steps of all sequences, for all threads of the CTA.
+__device__ __forceinline__ int64_t count_steps(const DecodeParams& p) {
+    if (!p.kv_lens) return (int64_t)steps_of(visible(p, 0)) * p.batch * p.n_kv;
+    __shared__ int64_t sums[kWarps];
+    int64_t x = 0;
+    for (int b = threadIdx.x; b < p.batch; b += kThreads) x += steps_of(visible(p, b));
 #pragma unroll
-    for (int off = 16; off; off >>= 1) {
-        x += __shfl_xor_sync(kFullMask, x, off);
-        y += __shfl_xor_sync(kFullMask, y, off);
-    }
-    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32][0] = x, sums[threadIdx.x / 32][1] = y;
+    for (int off = 16; off; off >>= 1) x += __shfl_xor_sync(kFullMask, x, off);
+    if (threadIdx.x % 32 == 0) sums[threadIdx.x / 32] = x;
     __syncthreads();
-    before = all = 0;
-    for (int w = 0; w < kWarps; ++w) before += sums[w][0], all += sums[w][1];
-    before *= p.n_kv, all *= p.n_kv;
-    __syncthreads();
+    x = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) x += sums[w];
+    return x * p.n_kv;
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_f16_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(b));
 }
 __device__ __forceinline__ void mma_f16_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                               uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
@@ -447,6 +432,9 @@ __device__ __forceinline__ void fetch(uint32_t to, const LanePlanes& from, int64
     }
 }
 
+// A warp is a worker: its run of steps may begin and end inside a (sequence, KV head) and pass over several.  What it has of
+// one that others work on too is a part for the merge kernel: part 2 i of worker i is what its run begins with, 2 i + 1
+// what it ends with.
 template <int D>
 __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(const DecodeParams p) {
     using S = Shape<D>;
@@ -454,22 +442,22 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
     extern __shared__ __align__(16) uint8_t smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, G = p.group;
-    int64_t before, all;
-    count_tiles(p, 0, before, all);
-    const int ctas = (int)min((int64_t)p.ctas, all);
-    if (blockIdx.x >= ctas) return;
-    int64_t at = share_start(blockIdx.x, all, ctas);
-    const int64_t end = share_start(blockIdx.x + 1, all, ctas);
-    // the sequence of the first tile
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, G = p.group, g = lane / 4, j = lane % 4;
+    const int64_t all = count_steps(p);
+    const int workers = (int)min((int64_t)p.workers, all);
+    const int worker = warp * gridDim.x + blockIdx.x;  // a launch of few spreads them over the SMs
+    if (worker >= workers) return;
+    int64_t at = share_start(worker, all, workers);
+    const int64_t end = share_start(worker + 1, all, workers);
+    // the sequence of the first step
     int b = 0;
-    int64_t first = 0;  // its first tile
+    int64_t first = 0;  // its first step
     if (!p.kv_lens) {
-        const int64_t n = (int64_t)tiles_of(visible(p, 0)) * p.n_kv;
+        const int64_t n = (int64_t)steps_of(visible(p, 0)) * p.n_kv;
         b = (int)(at / n), first = b * n;
     } else {
-        for (int b0 = 0;; b0 += 32) {  // every warp on its own
-            const int64_t n = b0 + lane < p.batch ? (int64_t)tiles_of(visible(p, b0 + lane)) * p.n_kv : 0;
+        for (int b0 = 0;; b0 += 32) {
+            const int64_t n = b0 + lane < p.batch ? (int64_t)steps_of(visible(p, b0 + lane)) * p.n_kv : 0;
             int64_t upto = n;
 #pragma unroll
             for (int off = 1; off < 32; off <<= 1) {
@@ -490,13 +478,11 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
     constexpr int kPiece = S::kScaleRow < 16 ? S::kScaleRow : 16;
     const LanePlanes planes{p.k_codes + lane * 16, p.v_codes + lane * 4, p.k_scales + lane * kPiece, p.v_scales + lane * kPiece};
     for (bool head = true; at < end; head = false) {
-        const int len = visible(p, b), n = tiles_of(len);
-        const int h = (int)((at - first) / n), tile = (int)((at - first) % n);
-        const int tiles = (int)min(end - at, (int64_t)(n - tile));
-        const int lo = tile * kTile, hi = min(len, lo + tiles * kTile);
+        const int len = visible(p, b), n = steps_of(len);
+        const int h = (int)((at - first) / n), step0 = (int)((at - first) % n);
+        const int steps = (int)min(end - at, (int64_t)(n - step0));
+        const int lo = step0 * kStep, hi = min(len, lo + steps * kStep);
         const int64_t bh = (int64_t)b * p.n_kv + h, rows = bh * p.max_seq;
-        const bool whole = tiles == n;
-        const int steps = (hi - lo + kStep - 1) / kStep;  // of the CTA; 0 without tokens
         auto prefetch = [&](int s, int slot) {
             const int valid = hi - lo - s * kStep;
             const uint32_t to = ring_at + slot * S::kStage;
@@ -504,197 +490,163 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
             else if (valid > 0) fetch<D>(to, planes, rows + lo + s * kStep, valid, lane);
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
+        __syncwarp();  // all lanes are done with what lies in the ring
 #pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) prefetch(warp + i * kWarps, i);
-        // one warp lays the queries out for all
+        for (int i = 0; i < kStages - 1; ++i) prefetch(i, i);
         Queries<D> q;
-        uint4* shared_q = reinterpret_cast<uint4*>(smem + S::kRing) + lane;
-        if (warp == 0) {
-            q.load(p, bh, lane);
-#pragma unroll
-            for (int i = 0; i < S::kGroups; ++i)
-                shared_q[i * 32] = make_uint4(q.even[i][0], q.odd[i][0], q.even[i][1], q.odd[i][1]);
-            shared_q[S::kGroups * 32] = make_uint4(q.sums[0], q.sums[S::kSpans - 1], __float_as_uint(q.factor[0]), __float_as_uint(q.factor[1]));
-        }
-        __syncthreads();
-        if (warp != 0) {
-#pragma unroll
-            for (int i = 0; i < S::kGroups; ++i) {
-                const uint4 x = shared_q[i * 32];
-                q.even[i][0] = x.x, q.odd[i][0] = x.y, q.even[i][1] = x.z, q.odd[i][1] = x.w;
-            }
-            const uint4 x = shared_q[S::kGroups * 32];
-            q.sums[0] = x.x, q.sums[S::kSpans - 1] = x.y, q.factor[0] = __uint_as_float(x.z), q.factor[1] = __uint_as_float(x.w);
-        }
+        q.load(p, bh, lane);
         Sums<D> a = {};
         a.top[0] = a.top[1] = -INFINITY;
         int slot = 0;
-        for (int s = warp; s < steps; s += kWarps) {
+        for (int t0 = lo, s = 0; t0 < hi; t0 += kStep, ++s) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
             __syncwarp();
             int next = slot + kStages - 1;
             if (next >= kStages) next -= kStages;
-            prefetch(s + (kStages - 1) * kWarps, next);
-            const int t0 = lo + s * kStep;
+            prefetch(s + kStages - 1, next);
             step<D>(ring + slot * S::kStage, hi - t0, q, a, lane, p.scores ? p.scores + rows * G + t0 : nullptr, p.max_seq, G);
             if (++slot == kStages) slot = 0;
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        // ---- the four warps' results, over the ring
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) a.l[c] += __shfl_xor_sync(kFullMask, a.l[c], off);
-        float* results = reinterpret_cast<float*>(smem);  // [warp][query][kResult]
-        float2* ml = reinterpret_cast<float2*>(results + kWarps * kMaxGroup * S::kResult);  // [warp][query]
-        float2* total = ml + kWarps * kMaxGroup;                                           // [query]
-        const int g = lane / 4, j = lane % 4;
-        __syncthreads();
-        if (g == 0) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-                ml[warp * kMaxGroup + 2 * j + c] = make_float2(a.top[c] == -INFINITY && a.l[c] == 0.f ? -INFINITY : a.ref[c], a.l[c]);
-        }
-        __syncthreads();
-        if (tid < kMaxGroup) {
-            float m = -INFINITY, l = 0.f;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * kMaxGroup + tid].x);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float2 x = ml[w * kMaxGroup + tid];
-                if (x.x != -INFINITY) l += x.y * exp2f(x.x - m);
-            }
-            total[tid] = make_float2(m, l);
+        // ---- the result, or a part of it
+        const bool whole = steps == n;
+        const int64_t part = (2 * (int64_t)worker + !head) * G;
+        if (lane == 0) {
+            if (step0 == 0) p.spans[bh].x = whole ? -1 : 2 * worker + !head;
+            if (step0 + steps == n) p.spans[bh].y = worker;
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            float m = -INFINITY;
+            float l = a.l[c];
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w * kMaxGroup + 2 * j + c].x);
-            const float mine = ml[warp * kMaxGroup + 2 * j + c].x, f = mine == -INFINITY ? 0.f : exp2f(mine - m);
-            float* row = results + (warp * kMaxGroup + 2 * j + c) * S::kResult;
-            const float even = f * exp2f((float)(24 - a.k)), odd = even * 0.0625f;
-            if (2 * j + c < G) {
+            for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(kFullMask, l, off);
+            const int h_q = 2 * j + c;
+            const bool mine = h_q < G;
+            const float even = exp2f((float)(24 - a.k)), odd = even * 0.0625f, inv = hi > lo ? 1.f / l : 0.f;
 #pragma unroll
-                for (int i = 0; i < S::kGroups; ++i) {
-                    const int d = (i / S::kSpanGroups) * S::R::kSpan + (g >> 1) * (S::R::kSpan / 4) + 8 * (i % S::kSpanGroups) + 4 * (g & 1);
-                    *reinterpret_cast<float4*>(row + d) =
-                        make_float4(a.o[i][0][c] * even, (a.o[i][0][c + 2] - a.o[i][0][c]) * odd, a.o[i][1][c] * even,
-                                    (a.o[i][1][c + 2] - a.o[i][1][c]) * odd);
+            for (int i = 0; i < S::kGroups; ++i) {
+                // the minima's sum of the group is with the lanes 2i + 1
+                const float sum = S::kSpans == 2 ? a.lo[c + 2 * (i / S::kSpanGroups)] : a.lo[c];
+                float y = __shfl_sync(kFullMask, sum, 8 * (i % S::kSpanGroups) + 4 + j);
+                if (S::kSpans == 1) y += __shfl_sync(kFullMask, a.lo2[c + 2], 8 * i + 4 + j);
+                const int d = (i / S::kSpanGroups) * S::R::kSpan + (g >> 1) * (S::R::kSpan / 4) + 8 * (i % S::kSpanGroups) + 4 * (g & 1);
+                const float4 o = make_float4(fmaf(a.o[i][0][c], even, y), fmaf(a.o[i][0][c + 2] - a.o[i][0][c], odd, y),
+                                             fmaf(a.o[i][1][c], even, y), fmaf(a.o[i][1][c + 2] - a.o[i][1][c], odd, y));
+                if (mine && whole) {
+                    const uint2 packed = make_uint2(float2_to_bf16x2(o.x * inv, o.y * inv), float2_to_bf16x2(o.z * inv, o.w * inv));
+                    *reinterpret_cast<uint2*>(p.out + (bh * G + h_q) * D + d) = packed;
+                } else if (mine) {
+                    *reinterpret_cast<float4*>(p.part_o + (part + h_q) * D + d) = o;
                 }
-                if ((g & 1) && (g >> 1) < S::kSpanGroups) {
-                    if (S::kSpans == 2) {
-                        row[D + (g >> 1)] = a.lo[c] * f;
-                        row[D + S::kSpanGroups + (g >> 1)] = a.lo[c + 2] * f;
-                    } else {
-                        row[D + (g >> 1)] = (a.lo[c] + a.lo2[c + 2]) * f;
-                    }
-                }
+            }
+            if (mine && g == 0) {
+                if (!whole) p.part_ml[part + h_q] = make_float2(a.ref[c], l);
+                else if (p.lse) p.lse[bh * G + h_q] = hi > lo ? a.ref[c] * kLn2 + logf(l) : -INFINITY;
             }
         }
-        __syncthreads();
-        const int64_t part = 2 * (int64_t)blockIdx.x + !head;
-        for (int i = tid; i < G * (D / 4); i += kThreads) {
-            const int q_at = i / (D / 4), d = i % (D / 4) * 4;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float* row = results + (w * kMaxGroup + q_at) * S::kResult;
-                const float4 x = *reinterpret_cast<const float4*>(row + d);
-                const float y = row[D + S::R::group_of_octet(d / 8)];
-                o.x += x.x + y, o.y += x.y + y, o.z += x.z + y, o.w += x.w + y;
-            }
-            const float2 t = total[q_at];
-            if (whole) {
-                const float inv = hi > lo ? 1.f / t.y : 0.f;
-                const uint2 packed = make_uint2(float2_to_bf16x2(hi > lo ? o.x * inv : 0.f, hi > lo ? o.y * inv : 0.f),
-                                                float2_to_bf16x2(hi > lo ? o.z * inv : 0.f, hi > lo ? o.w * inv : 0.f));
-                *reinterpret_cast<uint2*>(p.out + (bh * G + q_at) * D + d) = packed;
-                if (d == 0 && p.lse) p.lse[bh * G + q_at] = hi > lo ? t.x * kLn2 + logf(t.y) : -INFINITY;
-            } else {
-                *reinterpret_cast<float4*>(p.part_o + (part * G + q_at) * D + d) = o;
-                if (d == 0) p.part_ml[part * G + q_at] = t;
-            }
-        }
-        __syncthreads();
-        at += tiles;
-        if (h == p.n_kv - 1 && tile + tiles == n) first += (int64_t)n * p.n_kv, ++b;
+        at += steps;
+        if (h == p.n_kv - 1 && step0 + steps == n) first += (int64_t)n * p.n_kv, ++b;
     }
 }
 
-// The parts of (sequence, KV head) blockIdx.x that several CTAs worked on, query blockIdx.y: every fourth part a warp.
-template <int D>
-__global__ void __launch_bounds__(kThreads) kv4_merge_kernel(const DecodeParams p) {
+constexpr int kMergeWarps = 8;
+
+// The parts of a row (sequence, query head) that several workers have.  kWide: a CTA a row, every eighth part a warp; else
+// a warp a row.
+template <int D, bool kWide>
+__global__ void __launch_bounds__(32 * kMergeWarps) kv4_merge_kernel(const DecodeParams p) {
     constexpr int kPer = D / 32;  // dims of a lane
-    __shared__ float sums[kWarps][D], totals[kWarps];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int bh = blockIdx.x, b = bh / p.n_kv, h = blockIdx.y, G = p.group, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    int64_t before, all;
-    count_tiles(p, b, before, all);
-    const int n = tiles_of(visible(p, b));
-    const int64_t t0 = before + (int64_t)(bh % p.n_kv) * n;
-    const int ctas = (int)min((int64_t)p.ctas, all);
-    const int i0 = share_of(t0, all, ctas), i1 = share_of(t0 + n - 1, all, ctas);
-    if (i0 == i1) return;  // one CTA had all of it
-    // the first CTA's part is its last one, unless it begins with it
-    const int64_t head = 2 * (int64_t)i0 + (share_start(i0, all, ctas) < t0);
-    auto part = [&](int i) { return (i == i0 ? head : 2 * (int64_t)i) * G + h; };
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, G = p.group;
+    const int row = kWide ? blockIdx.x : blockIdx.x * kMergeWarps + warp;
+    if (row >= p.batch * p.n_kv * G) return;
+    const int bh = row / G, h = row % G;
+    const int2 span = p.spans[bh];
+    if (span.x < 0) return;  // one worker had all of it
+    const int i0 = span.x / 2, i1 = span.y;
+    auto part = [&](int i) { return (int64_t)(i == i0 ? span.x : 2 * i) * G + h; };
     float m = -INFINITY;
     for (int i = i0 + lane; i <= i1; i += 32) m = fmaxf(m, p.part_ml[part(i)].x);
 #pragma unroll
     for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
     float o[kPer] = {}, l = 0.f;
-#pragma unroll 4
-    for (int i = i0 + warp; i <= i1; i += kWarps) {
+#pragma unroll 8
+    for (int i = i0 + (kWide ? warp : 0); i <= i1; i += kWide ? kMergeWarps : 1) {
         const float2 x = p.part_ml[part(i)];
         const float f = exp2f(x.x - m);
         l += x.y * f;
-        const float* row = p.part_o + part(i) * D + lane * 2;
+        const float* from = p.part_o + part(i) * D + lane * 2;
 #pragma unroll
         for (int k = 0; k < kPer; k += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(row + 32 * k);
+            const float2 v = *reinterpret_cast<const float2*>(from + 32 * k);
             o[k] = fmaf(v.x, f, o[k]), o[k + 1] = fmaf(v.y, f, o[k + 1]);
         }
     }
+    if constexpr (kWide) {
+        __shared__ float sums[kMergeWarps][D], totals[kMergeWarps];
 #pragma unroll
-    for (int k = 0; k < kPer; k += 2) *reinterpret_cast<float2*>(&sums[warp][32 * k + 2 * lane]) = make_float2(o[k], o[k + 1]);
-    if (lane == 0) totals[warp] = l;
-    __syncthreads();
-    l = 0.f;
+        for (int k = 0; k < kPer; k += 2) *reinterpret_cast<float2*>(&sums[warp][32 * k + 2 * lane]) = make_float2(o[k], o[k + 1]);
+        if (lane == 0) totals[warp] = l;
+        __syncthreads();
+        l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) l += totals[w];
-    const int64_t row = (int64_t)bh * G + h;
-    for (int d = threadIdx.x; d < D; d += kThreads) {
-        float v = 0.f;
+        for (int w = 0; w < kMergeWarps; ++w) l += totals[w];
+        if (threadIdx.x < D) {
+            float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) v += sums[w][d];
-        p.out[row * D + d] = __float2bfloat16(v / l);
+            for (int w = 0; w < kMergeWarps; ++w) v += sums[w][threadIdx.x];
+            p.out[(int64_t)row * D + threadIdx.x] = __float2bfloat16(v / l);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kPer; k += 2)
+            *reinterpret_cast<uint32_t*>(p.out + (int64_t)row * D + 32 * k + 2 * lane) = float2_to_bf16x2(o[k] / l, o[k + 1] / l);
     }
-    if (threadIdx.x == 0 && p.lse) p.lse[row] = m * kLn2 + logf(l);
+    if ((kWide ? threadIdx.x : lane) == 0 && p.lse) p.lse[row] = m * kLn2 + logf(l);
 }
 
-// weights[t] += sum over the group of 2^(score - lse): a thread a token.
+// weights[t] += sum over the group of 2^(score - lse): a thread four neighbouring tokens.
 __global__ void __launch_bounds__(kThreads) kv4_weights_kernel(const DecodeParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t b = blockIdx.z, bh = b * p.n_kv + blockIdx.y;
-    const int len = visible(p, (int)b), t = blockIdx.x * kThreads + threadIdx.x;
+    const int len = visible(p, (int)b), t = (blockIdx.x * kThreads + threadIdx.x) * 4;
     if (t >= len) return;
     const float* x = p.scores + bh * p.group * p.max_seq + t;
-    float w = 0.f;
+    float* to = p.weights + bh * p.max_seq + t;
+    float w[4] = {};
+    const bool four = p.max_seq % 4 == 0 && (reinterpret_cast<uintptr_t>(p.weights) & 15) == 0;  // rows begin at 16 bytes
 #pragma unroll
-    for (int h = 0; h < kMaxGroup; ++h)
-        if (h < p.group) w += exp2f(x[h * p.max_seq] - p.lse[bh * p.group + h] * kLog2e);
-    p.weights[bh * p.max_seq + t] += w;
+    for (int h = 0; h < kMaxGroup; ++h) {
+        if (h >= p.group) continue;
+        const float l = p.lse[bh * p.group + h] * kLog2e;
+        float4 v = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        if (four) {  // tokens behind the length hold anything: they are not written
+            v = *reinterpret_cast<const float4*>(x + h * p.max_seq);
+        } else {
+            v.x = x[h * p.max_seq];
+            if (t + 1 < len) v.y = x[h * p.max_seq + 1];
+            if (t + 2 < len) v.z = x[h * p.max_seq + 2];
+            if (t + 3 < len) v.w = x[h * p.max_seq + 3];
+        }
+        w[0] += exp2f(v.x - l), w[1] += exp2f(v.y - l), w[2] += exp2f(v.z - l), w[3] += exp2f(v.w - l);
+    }
+    if (four && t + 3 < len) {
+        float4 v = *reinterpret_cast<float4*>(to);
+        v.x += w[0], v.y += w[1], v.z += w[2], v.w += w[3];
+        *reinterpret_cast<float4*>(to) = v;
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (t + k < len) to[k] += w[k];
+    }
 }
 
-// CTAs of a launch: as many as fit at a time, or one for every tile.
-int ctas_of(int64_t batch, int n_kv, int head_dim, int64_t max_seq) {
-    const int per_sm = head_dim == 64 ? Shape<64>::kPerSm : head_dim == 128 ? Shape<128>::kPerSm : Shape<256>::kPerSm;
-    const int64_t tiles = batch * n_kv * ((max_seq + kTile - 1) / kTile);
-    return (int)std::min(tiles, (int64_t)per_sm * sm_count());
+// Workers of a launch: as many warps as fit at a time, or one for every step.
+int workers_of(int64_t batch, int n_kv, int head_dim, int64_t max_seq) {
+    const int per_sm = kWarps * (head_dim == 64 ? Shape<64>::kPerSm : head_dim == 128 ? Shape<128>::kPerSm : Shape<256>::kPerSm);
+    const int64_t steps = batch * n_kv * ((max_seq + kStep - 1) / kStep);
+    return (int)std::min(steps, (int64_t)per_sm * sm_count());
 }
 
 inline size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
@@ -702,8 +654,8 @@ inline size_t round16(size_t n) { return (n + 15) & ~(size_t)15; }
 }  // namespace
 
 size_t kv4_decode_workspace_bytes(int64_t batch, int n_heads, int n_kv, int head_dim, int64_t max_seq, bool weighed) {
-    const size_t rows = 2 * (size_t)ctas_of(batch, n_kv, head_dim, max_seq) * (n_heads / n_kv + (n_heads % n_kv != 0));
-    return round16(rows * head_dim * sizeof(float)) + round16(rows * sizeof(float2)) +
+    const size_t rows = 2 * (size_t)workers_of(batch, n_kv, head_dim, max_seq) * (n_heads / n_kv + (n_heads % n_kv != 0));
+    return round16(rows * head_dim * sizeof(float)) + round16(rows * sizeof(float2)) + round16((size_t)batch * n_kv * sizeof(int2)) +
            (weighed ? round16((size_t)batch * n_heads * sizeof(float)) + round16((size_t)batch * n_heads * max_seq * sizeof(float)) : 0);
 }
 
@@ -716,12 +668,13 @@ cudaError_t launch_kv4_decode(const Kv4Cache& c, const void* q, void* out, float
     p.k_scales = (const uint8_t*)c.k_scales, p.v_scales = (const uint8_t*)c.v_scales;
     p.out = (__nv_bfloat16*)out, p.weights = weights;
     p.max_seq = max_seq, p.kv_lens = kv_lens, p.kv_len = (int)kv_len_uniform, p.batch = (int)batch;
-    p.n_kv = n_kv, p.group = n_heads / n_kv, p.ctas = ctas_of(batch, n_kv, head_dim, max_seq);
+    p.n_kv = n_kv, p.group = n_heads / n_kv, p.workers = workers_of(batch, n_kv, head_dim, max_seq);
     p.scale_log2 = scale * kLog2e;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    const size_t rows = 2 * (size_t)p.ctas * p.group;
+    const size_t rows = 2 * (size_t)p.workers * p.group;
     p.part_o = (float*)ws, ws += round16(rows * head_dim * sizeof(float));
     p.part_ml = (float2*)ws, ws += round16(rows * sizeof(float2));
+    p.spans = (int2*)ws, ws += round16((size_t)batch * n_kv * sizeof(int2));
     if (weights) {
         if (!lse) lse = (float*)ws;
         ws += round16((size_t)batch * n_heads * sizeof(float));
@@ -732,11 +685,17 @@ cudaError_t launch_kv4_decode(const Kv4Cache& c, const void* q, void* out, float
         constexpr int D = decltype(d)::value;
         cudaError_t e = set_max_dynamic_smem_once<kv4_decode_kernel<D>>(Shape<D>::kSmem);
         if (e != cudaSuccess) return e;
-        e = launch_chained(kv4_decode_kernel<D>, dim3(p.ctas), kThreads, Shape<D>::kSmem, stream, p);
-        if (e == cudaSuccess && p.ctas > 1)
-            e = launch_chained(kv4_merge_kernel<D>, dim3((unsigned)(batch * n_kv), p.group), kThreads, 0, stream, p);
+        e = launch_chained(kv4_decode_kernel<D>, dim3((p.workers + kWarps - 1) / kWarps), kThreads, Shape<D>::kSmem, stream, p);
+        if (e == cudaSuccess && p.workers > 1) {
+            // a row has about workers * group / rows parts
+            const int64_t n = batch * n_heads;
+            e = p.workers * (int64_t)p.group >= 8 * n
+                    ? launch_chained(kv4_merge_kernel<D, true>, dim3((unsigned)n), 32 * kMergeWarps, 0, stream, p)
+                    : launch_chained(kv4_merge_kernel<D, false>, dim3((unsigned)((n + kMergeWarps - 1) / kMergeWarps)), 32 * kMergeWarps, 0,
+                                     stream, p);
+        }
         if (e == cudaSuccess && weights)
-            e = launch_chained(kv4_weights_kernel, dim3((unsigned)((max_seq + kThreads - 1) / kThreads), n_kv, (unsigned)batch),
+            e = launch_chained(kv4_weights_kernel, dim3((unsigned)((max_seq + 4 * kThreads - 1) / (4 * kThreads)), n_kv, (unsigned)batch),
                                kThreads, 0, stream, p);
         return e;
     });
