@@ -548,13 +548,13 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
     }
 }
 
-constexpr int kMergeWarps = 8;
+constexpr int kMergeWarps = 8, kMergeParts = 256;
 
 // The parts of a row (sequence, query head) that several workers have.  kWide: a CTA a row, every eighth part a warp; else
 // a warp a row.
 template <int D, bool kWide>
 __global__ void __launch_bounds__(32 * kMergeWarps) kv4_merge_kernel(const DecodeParams p) {
-    constexpr int kPer = D / 32;  // dims of a lane
+    constexpr int kPer = D / 32;  // dims of a lane: neighbours
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, G = p.group;
@@ -563,29 +563,44 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_merge_kernel(const Decod
     const int bh = row / G, h = row % G;
     const int2 span = p.spans[bh];
     if (span.x < 0) return;  // one worker had all of it
-    const int i0 = span.x / 2, i1 = span.y;
-    auto part = [&](int i) { return (int64_t)(i == i0 ? span.x : 2 * i) * G + h; };
+    const int i0 = span.x / 2, n = span.y - i0 + 1;
+    auto part = [&](int r) { return (int64_t)(r == 0 ? span.x : 2 * (i0 + r)) * G + h; };
     float m = -INFINITY;
-    for (int i = i0 + lane; i <= i1; i += 32) m = fmaxf(m, p.part_ml[part(i)].x);
+    for (int r = kWide ? threadIdx.x : lane; r < n; r += kWide ? 32 * kMergeWarps : 32) m = fmaxf(m, p.part_ml[part(r)].x);
 #pragma unroll
     for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
     float o[kPer] = {}, l = 0.f;
-#pragma unroll 8
-    for (int i = i0 + (kWide ? warp : 0); i <= i1; i += kWide ? kMergeWarps : 1) {
-        const float2 x = p.part_ml[part(i)];
-        const float f = exp2f(x.x - m);
-        l += x.y * f;
-        const float* from = p.part_o + part(i) * D + lane * 2;
+    auto add = [&](int r, float f) {
+        const float* from = p.part_o + part(r) * D + lane * kPer;
 #pragma unroll
         for (int k = 0; k < kPer; k += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(from + 32 * k);
+            const float2 v = *reinterpret_cast<const float2*>(from + k);
             o[k] = fmaf(v.x, f, o[k]), o[k + 1] = fmaf(v.y, f, o[k + 1]);
         }
-    }
+    };
     if constexpr (kWide) {
-        __shared__ float sums[kMergeWarps][D], totals[kMergeWarps];
+        __shared__ float sums[kMergeWarps][D], totals[kMergeWarps], tops[kMergeWarps], factor[kMergeParts];
+        if (lane == 0) tops[warp] = m;
+        __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kPer; k += 2) *reinterpret_cast<float2*>(&sums[warp][32 * k + 2 * lane]) = make_float2(o[k], o[k + 1]);
+        for (int w = 0; w < kMergeWarps; ++w) m = fmaxf(m, tops[w]);
+        for (int r0 = 0; r0 < n; r0 += kMergeParts) {  // the factors first, so that the rows' loads wait for nothing
+            const int count = min(kMergeParts, n - r0);
+            if (r0) __syncthreads();
+            if (threadIdx.x < count) {
+                const float2 x = p.part_ml[part(r0 + threadIdx.x)];
+                const float f = exp2f(x.x - m);
+                factor[threadIdx.x] = f;
+                l += x.y * f;
+            }
+            __syncthreads();
+#pragma unroll 8
+            for (int r = warp; r < count; r += kMergeWarps) add(r0 + r, factor[r]);
+        }
+#pragma unroll
+        for (int off = 16; off; off >>= 1) l += __shfl_xor_sync(kFullMask, l, off);
+#pragma unroll
+        for (int k = 0; k < kPer; k += 2) *reinterpret_cast<float2*>(&sums[warp][kPer * lane + k]) = make_float2(o[k], o[k + 1]);
         if (lane == 0) totals[warp] = l;
         __syncthreads();
         l = 0.f;
@@ -598,9 +613,16 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_merge_kernel(const Decod
             p.out[(int64_t)row * D + threadIdx.x] = __float2bfloat16(v / l);
         }
     } else {
+#pragma unroll 4
+        for (int r = 0; r < n; ++r) {
+            const float2 x = p.part_ml[part(r)];
+            const float f = exp2f(x.x - m);
+            l += x.y * f;
+            add(r, f);
+        }
 #pragma unroll
         for (int k = 0; k < kPer; k += 2)
-            *reinterpret_cast<uint32_t*>(p.out + (int64_t)row * D + 32 * k + 2 * lane) = float2_to_bf16x2(o[k] / l, o[k + 1] / l);
+            *reinterpret_cast<uint32_t*>(p.out + (int64_t)row * D + kPer * lane + k) = float2_to_bf16x2(o[k] / l, o[k + 1] / l);
     }
     if ((kWide ? threadIdx.x : lane) == 0 && p.lse) p.lse[row] = m * kLn2 + logf(l);
 }

@@ -38,10 +38,22 @@ __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
 }
 // What lies at `p` in the shared memory of the cluster's CTA `rank`.
-__device__ __forceinline__ uint32_t load_remote(const uint32_t* p, int rank) {
-    uint32_t at, x;
+__device__ __forceinline__ uint32_t remote_address(const void* p, int rank) {
+    uint32_t at;
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+    return at;
+}
+__device__ __forceinline__ uint32_t load_remote(const uint32_t* p, int rank) {
+    uint32_t x;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(remote_address(p, rank)) : "memory");
+    return x;
+}
+__device__ __forceinline__ uint4 load_remote4(const uint32_t* p, int rank) {
+    uint4 x;
+    asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                 : "r"(remote_address(p, rank))
+                 : "memory");
     return x;
 }
 
@@ -118,19 +130,26 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(const SelectParams 
         }
         if (C > 1) cluster_barrier();
         else __syncthreads();
-        // the digit where the count from above reaches `left`: thread i holds bins 2i and 2i + 1 from the top
-        const uint32_t hi_bin = kBins - 1 - 2 * tid;
-        uint32_t a = 0, c = 0;
-        if (C > 1) {
-            for (int r = 0; r < C; ++r) a += load_remote(&bins[hi_bin], r), c += load_remote(&bins[hi_bin - 1], r);
-        } else {
-            a = bins[hi_bin], c = bins[hi_bin - 1];
+        // the digit where the count from above reaches `left`: each of 512 threads has four bins, from the top
+        const int low = kBins - 4 - 4 * tid;
+        uint4 x4 = make_uint4(0, 0, 0, 0);
+        if (tid < kBins / 4) {
+            if (C == 1) x4 = *reinterpret_cast<const uint4*>(&bins[low]);
+            else
+                for (int r = 0; r < C; ++r) {
+                    const uint4 y = load_remote4(&bins[low], r);
+                    x4.x += y.x, x4.y += y.y, x4.z += y.z, x4.w += y.w;
+                }
         }
-        const uint32_t upto = (uint32_t)block_scan(a + c, sh.warps), before = upto - a - c;
+        const uint32_t mine4 = x4.x + x4.y + x4.z + x4.w;
+        const uint32_t upto = (uint32_t)block_scan(mine4, sh.warps), before = upto - mine4;
         if (before < (uint32_t)left && upto >= (uint32_t)left) {
-            const bool upper = before + a >= (uint32_t)left;
-            sh.digit = upper ? hi_bin : hi_bin - 1;
-            sh.above = upper ? before : before + a;
+            const uint32_t c[4] = {x4.w, x4.z, x4.y, x4.x};
+            uint32_t above = before;
+            int k = 0;
+            while (above + c[k] < (uint32_t)left) above += c[k++];
+            sh.digit = low + 3 - k;
+            sh.above = above;
         }
         __syncthreads();
         prefix |= sh.digit << shift;
@@ -165,7 +184,7 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(const SelectParams 
     if (C > 1) cluster_barrier();  // nobody leaves while its shared memory is read
 }
 
-constexpr int kMoveRows = 64, kMoveThreads = 256;
+constexpr int kMoveThreads = 256, kMoveBatch = 4;  // a thread's loads in flight
 
 struct MoveParams {
     EvictPlanes planes;
@@ -174,45 +193,38 @@ struct MoveParams {
     int keep;
 };
 
-// 64 kept rows of a (sequence, KV head), all planes.
+// A run of a plane's kept rows of a (sequence, KV head), 16 (or 8) bytes a load.
 template <class Unit>
-__device__ __forceinline__ void move_rows(const uint8_t* src, uint8_t* dst, const int32_t* from, int rows, int row_bytes) {
-    const unsigned units = row_bytes / sizeof(Unit), all = rows * units;
-    constexpr int kBatch = 4;  // loads of a thread in flight
-    for (unsigned i0 = threadIdx.x; i0 < all; i0 += kBatch * kMoveThreads) {
-        Unit x[kBatch];
+__device__ __forceinline__ void move_rows(const MoveParams& p, int plane, int64_t bh) {
+    const unsigned row_bytes = p.planes.row_bytes[plane], units = row_bytes / sizeof(Unit);
+    const uint8_t* src = static_cast<const uint8_t*>(p.planes.src[plane]) + bh * p.max_seq * row_bytes;
+    uint8_t* dst = static_cast<uint8_t*>(p.planes.dst[plane]) + bh * p.max_seq_out * row_bytes;
+    const int32_t* kept = p.kept + bh * p.keep;
+    const int64_t all = (int64_t)p.keep * units, first = (int64_t)blockIdx.x * kMoveThreads * kMoveBatch + threadIdx.x;
+    int32_t from[kMoveBatch];
+    unsigned at[kMoveBatch];
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const unsigned i = i0 + k * kMoveThreads, r = i / units;
-            if (i < all) x[k] = *reinterpret_cast<const Unit*>(src + (int64_t)from[r] * row_bytes + (i - r * units) * sizeof(Unit));
-        }
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-            const unsigned i = i0 + k * kMoveThreads;
-            if (i < all) *reinterpret_cast<Unit*>(dst + (int64_t)i * sizeof(Unit)) = x[k];
-        }
+    for (int k = 0; k < kMoveBatch; ++k) {
+        const int64_t i = first + k * kMoveThreads;
+        const int64_t r = i >> 32 ? i / units : (unsigned)i / units;
+        at[k] = (unsigned)(i - r * units);
+        from[k] = i < all ? kept[r] : -1;
     }
+    Unit x[kMoveBatch];
+#pragma unroll
+    for (int k = 0; k < kMoveBatch; ++k)
+        if (from[k] >= 0) x[k] = *reinterpret_cast<const Unit*>(src + (int64_t)from[k] * row_bytes + at[k] * sizeof(Unit));
+#pragma unroll
+    for (int k = 0; k < kMoveBatch; ++k)
+        if (from[k] >= 0) *reinterpret_cast<Unit*>(dst + (first + k * kMoveThreads) * sizeof(Unit)) = x[k];
 }
 
+// Grid: (runs of rows, plane, sequence and KV head).
 __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const MoveParams p) {
-    __shared__ int32_t from[kMoveRows];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t bh = blockIdx.y;
-    const int first = blockIdx.x * kMoveRows, most = min(kMoveRows, p.keep - first);
-    bool there = false;
-    if (threadIdx.x < most) {
-        from[threadIdx.x] = p.kept[bh * p.keep + first + threadIdx.x];
-        there = from[threadIdx.x] >= 0;
-    }
-    const int rows = __syncthreads_count(there);  // those behind the kept ones come last
-    for (int i = 0; i < p.planes.n; ++i) {
-        const int bytes = p.planes.row_bytes[i];
-        const uint8_t* src = static_cast<const uint8_t*>(p.planes.src[i]) + bh * p.max_seq * bytes;
-        uint8_t* dst = static_cast<uint8_t*>(p.planes.dst[i]) + (bh * p.max_seq_out + first) * bytes;
-        if (bytes % 16 == 0) move_rows<uint4>(src, dst, from, rows, bytes);
-        else move_rows<uint2>(src, dst, from, rows, bytes);
-    }
+    if (p.planes.row_bytes[blockIdx.y] % 16 == 0) move_rows<uint4>(p, blockIdx.y, blockIdx.z);
+    else move_rows<uint2>(p, blockIdx.y, blockIdx.z);
 }
 
 }  // namespace
@@ -251,8 +263,11 @@ cudaError_t launch_kv_evict(const EvictPlanes& planes, const float* weights, flo
     if (e != cudaSuccess) return e;
     MoveParams m;
     m.planes = planes, m.kept = kept, m.max_seq = max_seq, m.max_seq_out = max_seq_out, m.keep = (int)keep;
-    return launch_chained(kv_move_kernel, dim3((unsigned)((keep + kMoveRows - 1) / kMoveRows), (unsigned)(batch * n_kv)), kMoveThreads,
-                          0, stream, m);
+    int64_t units = 1;
+    for (int i = 0; i < planes.n; ++i) units = std::max(units, keep * (planes.row_bytes[i] / (planes.row_bytes[i] % 16 ? 8 : 16)));
+    const int64_t per = kMoveThreads * kMoveBatch;
+    return launch_chained(kv_move_kernel, dim3((unsigned)((units + per - 1) / per), planes.n, (unsigned)(batch * n_kv)), kMoveThreads, 0,
+                          stream, m);
 }
 
 }  // namespace rt
