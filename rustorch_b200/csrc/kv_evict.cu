@@ -14,7 +14,7 @@
 namespace rt {
 namespace {
 
-constexpr int kThreads = 1024, kWarps = kThreads / 32, kBins = 2 * kThreads, kPasses = 3;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 2048, kPasses = 3;
 constexpr int kMostCluster = 8;
 constexpr int kHeld = 32 * 1024;  // candidates of a CTA that its shared memory holds; longer runs are read again instead
 
@@ -75,11 +75,87 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t x, uint64_t* warps) {
     __syncthreads();
     if (lane == 31) warps[warp] = x;
     __syncthreads();
-    static_assert(kWarps == 32, "a warp adds up the warps' sums");
-    uint64_t before = lane < warp ? warps[lane] : 0;
 #pragma unroll
-    for (int off = 16; off; off >>= 1) before += __shfl_xor_sync(kFullMask, before, off);
-    return x + before;
+    for (int w = 0; w < kWarps; ++w) x += w < warp ? warps[w] : 0;
+    return x;
+}
+
+// Of this CTA's candidates (load(0) to load(count - 1), the first of them the row's candidate `first`), those that belong
+// to the cluster's `want` heaviest go to their places.
+template <class Load>
+__device__ __forceinline__ void choose(SelectShared& sh, int C, int rank, int count, int first, int want, int32_t* kept, float* w_out,
+                                       Load&& load) {
+    const int tid = threadIdx.x;
+    constexpr int kBatch = 4;  // loads of a thread in flight
+    uint32_t prefix = 0, mask = 0;
+    int left = want;  // of the candidates with the prefix
+#pragma unroll
+    for (int pass = 0; pass < kPasses; ++pass) {
+        constexpr int shifts[kPasses] = {21, 10, 0}, widths[kPasses] = {11, 11, 10};
+        const int shift = shifts[pass];
+        const uint32_t digit = (1u << widths[pass]) - 1;
+        uint32_t* bins = sh.bins[pass];
+        for (int i0 = tid; i0 < count; i0 += kBatch * kThreads) {
+            uint32_t k[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) k[u] = order_key(load(min(i0 + u * kThreads, count - 1)));
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u)
+                if (i0 + u * kThreads < count && (k[u] & mask) == prefix) atomicAdd(&bins[k[u] >> shift & digit], 1u);
+        }
+        if (C > 1) cluster_barrier();
+        else __syncthreads();
+        // the digit where the count from above reaches `left`: a thread has four bins, from the top
+        static_assert(kBins == 4 * kThreads, "four bins a thread");
+        const int low = kBins - 4 - 4 * tid;
+        uint4 u = *reinterpret_cast<const uint4*>(&bins[low]);
+        for (int r = 1; r < C; ++r) {
+            const uint4 x = load_remote4(&bins[low], rank + r < C ? rank + r : rank + r - C);
+            u.x += x.x, u.y += x.y, u.z += x.z, u.w += x.w;
+        }
+        const uint32_t all = u.x + u.y + u.z + u.w;
+        const uint32_t upto = (uint32_t)block_scan(all, sh.warps), before = upto - all;
+        if (before < (uint32_t)left && upto >= (uint32_t)left) {
+            uint32_t above = before;
+            int at = 3;
+            if (above + u.w < (uint32_t)left) above += u.w, at = 2;
+            if (at == 2 && above + u.z < (uint32_t)left) above += u.z, at = 1;
+            if (at == 1 && above + u.y < (uint32_t)left) above += u.y, at = 0;
+            sh.digit = low + at;
+            sh.above = above;
+        }
+        __syncthreads();
+        prefix |= sh.digit << shift;
+        mask |= digit << shift;
+        left -= (int)sh.above;
+    }
+    // In order: larger keys, and the first `left` equal ones.  A thread has an odd number of neighbours, so that a warp's
+    // reads lie in different banks.
+    const int each = ((count + kThreads - 1) / kThreads) | 1;
+    const int begin = min(count, tid * each), end = min(count, begin + each);
+    uint32_t gt = 0, eq = 0;
+#pragma unroll 4
+    for (int i = begin; i < end; ++i) {
+        const uint32_t k = order_key(load(i));
+        gt += k > prefix, eq += k == prefix;
+    }
+    const uint64_t upto = block_scan((uint64_t)gt << 32 | eq, sh.warps);
+    gt = (uint32_t)(upto >> 32) - gt, eq = (uint32_t)upto - eq;  // of the threads before
+    if (C > 1) {
+        if (tid == kThreads - 1) sh.larger = (uint32_t)(upto >> 32), sh.equal = (uint32_t)upto;
+        cluster_barrier();
+        for (int r = 0; r < rank; ++r) gt += load_remote(&sh.larger, r), eq += load_remote(&sh.equal, r);
+    }
+#pragma unroll 4
+    for (int i = begin; i < end; ++i) {
+        const float v = load(i);
+        const uint32_t k = order_key(v);
+        if (k > prefix || (k == prefix && eq < (uint32_t)left)) {
+            const uint32_t to = gt + min(eq, (uint32_t)left);
+            kept[to] = first + i, w_out[to] = v;
+        }
+        gt += k > prefix, eq += k == prefix;
+    }
 }
 
 __global__ void __launch_bounds__(kThreads) kv_select_kernel(const SelectParams p) {
@@ -87,7 +163,6 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(const SelectParams 
     SelectShared& sh = *reinterpret_cast<SelectShared*>(smem);
     float* held = reinterpret_cast<float*>(smem + sizeof(SelectShared));
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int tid = threadIdx.x, C = p.cluster, rank = blockIdx.x % C, h = blockIdx.x / C;
     const int64_t b = blockIdx.y, bh = b * p.n_kv + h;
     const int len = (int)max((int64_t)0, min(p.kv_lens ? (int64_t)p.kv_lens[b] : (int64_t)p.kv_len, p.max_seq));
@@ -111,76 +186,11 @@ __global__ void __launch_bounds__(kThreads) kv_select_kernel(const SelectParams 
     const int run = (n + C - 1) / C, first = min(n, rank * run), count = min(n, first + run) - first;
     const float* x = w + first;
     for (int i = tid; i < kPasses * kBins; i += kThreads) sh.bins[0][i] = 0;
-    if (run <= p.held) {
+    if (run <= p.held)
         for (int i = tid; i < count; i += kThreads) held[i] = x[i];
-        x = held;
-    }
     __syncthreads();
-    uint32_t prefix = 0, mask = 0;
-    int left = want;  // of the candidates with the prefix
-#pragma unroll
-    for (int pass = 0; pass < kPasses; ++pass) {
-        constexpr int shifts[kPasses] = {21, 10, 0}, widths[kPasses] = {11, 11, 10};
-        const int shift = shifts[pass];
-        const uint32_t digit = (1u << widths[pass]) - 1;
-        uint32_t* bins = sh.bins[pass];
-        for (int i = tid; i < count; i += kThreads) {
-            const uint32_t k = order_key(x[i]);
-            if ((k & mask) == prefix) atomicAdd(&bins[k >> shift & digit], 1u);
-        }
-        if (C > 1) cluster_barrier();
-        else __syncthreads();
-        // the digit where the count from above reaches `left`: each of 512 threads has four bins, from the top
-        const int low = kBins - 4 - 4 * tid;
-        uint4 x4 = make_uint4(0, 0, 0, 0);
-        if (tid < kBins / 4) {
-            if (C == 1) x4 = *reinterpret_cast<const uint4*>(&bins[low]);
-            else
-                for (int r = 0; r < C; ++r) {
-                    const uint4 y = load_remote4(&bins[low], r);
-                    x4.x += y.x, x4.y += y.y, x4.z += y.z, x4.w += y.w;
-                }
-        }
-        const uint32_t mine4 = x4.x + x4.y + x4.z + x4.w;
-        const uint32_t upto = (uint32_t)block_scan(mine4, sh.warps), before = upto - mine4;
-        if (before < (uint32_t)left && upto >= (uint32_t)left) {
-            const uint32_t c[4] = {x4.w, x4.z, x4.y, x4.x};
-            uint32_t above = before;
-            int k = 0;
-            while (above + c[k] < (uint32_t)left) above += c[k++];
-            sh.digit = low + 3 - k;
-            sh.above = above;
-        }
-        __syncthreads();
-        prefix |= sh.digit << shift;
-        mask |= digit << shift;
-        left -= (int)sh.above;
-    }
-    // In order: larger keys, and the first `left` equal ones.  A thread has an odd number of neighbours, so that a warp's
-    // reads lie in different banks.
-    const int each = ((count + kThreads - 1) / kThreads) | 1;
-    const int begin = min(count, tid * each), end = min(count, begin + each);
-    uint32_t gt = 0, eq = 0;
-    for (int i = begin; i < end; ++i) {
-        const uint32_t k = order_key(x[i]);
-        gt += k > prefix, eq += k == prefix;
-    }
-    const uint64_t upto = block_scan((uint64_t)gt << 32 | eq, sh.warps);
-    gt = (uint32_t)(upto >> 32) - gt, eq = (uint32_t)upto - eq;  // of the threads before
-    if (C > 1) {
-        if (tid == kThreads - 1) sh.larger = (uint32_t)(upto >> 32), sh.equal = (uint32_t)upto;
-        cluster_barrier();
-        for (int r = 0; r < rank; ++r) gt += load_remote(&sh.larger, r), eq += load_remote(&sh.equal, r);
-    }
-    for (int i = begin; i < end; ++i) {
-        const float v = x[i];
-        const uint32_t k = order_key(v);
-        if (k > prefix || (k == prefix && eq < (uint32_t)left)) {
-            const uint32_t to = gt + min(eq, (uint32_t)left);
-            kept[to] = first + i, w_out[to] = v;
-        }
-        gt += k > prefix, eq += k == prefix;
-    }
+    if (run <= p.held) choose(sh, C, rank, count, first, want, kept, w_out, [&](int i) { return held[i]; });
+    else choose(sh, C, rank, count, first, want, kept, w_out, [&](int i) { return x[i]; });
     if (C > 1) cluster_barrier();  // nobody leaves while its shared memory is read
 }
 
@@ -237,7 +247,8 @@ cudaError_t launch_kv_evict(const EvictPlanes& planes, const float* weights, flo
     s.weights = weights, s.weights_out = weights_out, s.kept = kept, s.lens_out = lens_out;
     s.max_seq = max_seq, s.max_seq_out = max_seq_out, s.kv_lens = kv_lens, s.kv_len = (int)kv_len_uniform;
     s.n_kv = n_kv, s.keep = (int)keep, s.recent = (int)recent;
-    // More CTAs a head while each keeps 2048 candidates and all find an SM.
+    // More CTAs a head while each keeps 2048 candidates and all find an SM (29,745 candidates of 8 heads: 28.5 us on the device with
+    // one, 19.2 with four, 19.5 with eight).
     const int64_t longest = kv_lens ? max_seq : kv_len_uniform;
     int cluster = 1;
     while (cluster < kMostCluster && longest >= 2 * cluster * 2048 && 2 * cluster * batch * n_kv <= sm_count()) cluster *= 2;
@@ -252,13 +263,13 @@ cudaError_t launch_kv_evict(const EvictPlanes& planes, const float* weights, flo
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster, attr[1].val.clusterDim.y = 1, attr[1].val.clusterDim.z = 1;
+    // Not chained to the kernel ahead: CTAs that became resident beside the last ones of that kernel crowded a few SMs (8 heads
+    // of 30,001 tokens, calls back to back: 37 us a call chained, 29 not).
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 2;
+    cfg.numAttrs = 1;
     e = cudaLaunchKernelEx(&cfg, kv_select_kernel, s);
     if (e != cudaSuccess) return e;
     MoveParams m;
