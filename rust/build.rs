@@ -7,7 +7,7 @@
 use std::path::PathBuf;
 use std::process::Command;
 
-const SOURCES: &[&str] = &["api.cu", "decode.cu", "decode_tc.cu", "prefill_simt.cu", "prefill_tc.cu", "tc_selftest.cu", "decode_static.cu", "backward_simt.cu", "backward_tc.cu", "backward_tcgen05.cu", "api_cache.cu", "kv4_rows.cu", "kv4_decode.cu", "kv_weigh.cu", "kv_evict.cu"];
+const SOURCES: &[&str] = &["api.cu", "decode.cu", "decode_tc.cu", "prefill_simt.cu", "prefill_tc.cu", "tc_selftest.cu", "decode_static.cu", "backward_simt.cu", "backward_tc.cu", "backward_tcgen05.cu", "api_cache.cu", "kv4_rows.cu", "kv4_decode.cu", "kv_weigh.cu", "kv_weigh_tc.cu", "kv_evict.cu"];
 
 fn main() {
     if std::env::var("CARGO_FEATURE_CUDA").is_err() {

@@ -19,7 +19,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 LIB_PATH = os.path.join(PKG_DIR, "librustorch_attn.so")
 BINDING_PATH = os.path.join(PKG_DIR, "_torch_binding.so")
 BINDING_SOURCE = os.path.join(CSRC, "torch_binding.cpp")
-SOURCES = ["api.cu", "decode.cu", "decode_tc.cu", "prefill_simt.cu", "prefill_tc.cu", "tc_selftest.cu", "decode_static.cu", "backward_simt.cu", "backward_tc.cu", "backward_tcgen05.cu", "api_cache.cu", "kv4_rows.cu", "kv4_decode.cu", "kv_weigh.cu", "kv_evict.cu"]
+SOURCES = ["api.cu", "decode.cu", "decode_tc.cu", "prefill_simt.cu", "prefill_tc.cu", "tc_selftest.cu", "decode_static.cu", "backward_simt.cu", "backward_tc.cu", "backward_tcgen05.cu", "api_cache.cu", "kv4_rows.cu", "kv4_decode.cu", "kv_weigh.cu", "kv_weigh_tc.cu", "kv_evict.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

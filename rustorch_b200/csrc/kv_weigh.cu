@@ -16,6 +16,7 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kBlock = 64;  // query rows in shared memory at a time
+constexpr int kTensorRows = 64;  // rows of a KV head from which kv_weigh_tc.cu's kernel is taken
 
 struct WeighParams {
     const __nv_bfloat16 *q, *k;
@@ -158,6 +159,11 @@ cudaError_t launch_kv_weigh(const void* q, const void* k_cache, const float* lse
     p.n_kv = n_kv, p.group = n_heads / n_kv, p.scale_log2 = scale * kLog2e;
     const int64_t longest = kv_lens ? max_seq : kv_len_uniform;
     if (longest == 0) return cudaSuccess;
+    if (p.group * seq_q >= kTensorRows) {
+        const cudaError_t e = launch_kv_weigh_tc(q, k_cache, lse, weights, batch, n_heads, n_kv, seq_q, head_dim, max_seq, longest, kv_lens,
+                                                 kv_len_uniform, scale, stream);
+        if (e != cudaErrorNotSupported) return e;
+    }
     return for_head_dim(head_dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
         using S = WeighShape<D>;
