@@ -88,7 +88,7 @@ const char* rt_attn_error_string(int status);
  * Reads (and clears) the device-side status word of the current device: 0 = clean,
  * otherwise a code identifying which bounded wait inside a kernel gave up (101-114: a barrier of
  * the prefill kernel, 301: a TMA stage of the decode kernel, 401: a peer's record in
- * rt_attn_merge_records_after).  Synchronises the device.  Returns RT_OK, a cudaError_t, or RT_ERR_DEVICE_TIMEOUT when *status != 0.
+ * rt_attn_merge_records_after, 501-504: a barrier of rt_kv_weigh_bf16's tensor-core kernel).  Synchronises the device.  Returns RT_OK, a cudaError_t, or RT_ERR_DEVICE_TIMEOUT when *status != 0.
  */
 int rt_attn_device_status(int* status);
 
@@ -541,7 +541,9 @@ size_t rt_kv4_decode_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_k
  * Batched single-token GQA decode over a 4-bit cache: softmax(scale * q K^T) V of the values the codes stand for.
  *   q, out : bf16 [B,Hq,D];  lse : NULL or f32 [B,Hq];  kv_lens : device int32 [B] (clamped to max_seq), or NULL
  *   for kv_len_uniform;  scale <= 0 selects 1/sqrt(D).  Hq/Hkv from 1 to 8.  A sequence of length 0 gives
- *   out = 0, lse = -inf.
+ *   out = 0, lse = -inf.  Queries up to 2^100 in magnitude; a NaN or an infinity in a query makes its row NaN.
+ *   lse is as exact as f32 sums are; out is rounded to bf16 from sums of probabilities with 11 bits.  How a sequence
+ *   is cut depends on the other sequences' lengths, so that the last bit of a result does too.
  *   weights : NULL or f32 [B,Hkv,max_seq]; weights[b,h,t] += the sum over the query heads of KV head h of the
  *   softmax weight of token t < kv_len (what rt_kv_evict chooses by).
  */

@@ -209,7 +209,7 @@ struct Sums {
     float o[D / 32][2][4];       // [group][0-1, 2-3 of a lane's four dims]: sum p scale c 2^(k - 24), {q 2j, 2j+1} x {c0, c0 + 16 c1}
     float lo[4], lo2[4];         // sum p * lo: row 2i + 1 = group i; see `step` for which of the rows count
     float ref[2], top[2], l[2];  // p = 2^(score - ref); running maximum; sum of p (this lane's tokens)
-    int k;                       // scales are held times 2^k: the largest so far lies in [1/2, 1), k is 15 at most
+    int k;                       // scales are held times 2^k: the largest so far lies in [1/2, 1) (the format's are below 2^14), k <= 15
     uint32_t scale_limit;        // the largest f16 pattern for which k stands
 };
 constexpr float kBase = 15.f - kLazy;  // log2 of what p is held times: the largest reaches 2^15
@@ -305,7 +305,7 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
         big = __reduce_max_sync(kFullMask, big);
         float grow = 1.f;  // of the scales
         if (big > a.scale_limit) {
-            const int e = (int)(__float_as_uint(low_half(big)) >> 23) - 127, k = min(-1 - e, 15);
+            const int e = (int)(__float_as_uint(low_half(big)) >> 23) - 127, k = max(-14, min(-1 - e, 15));
             grow = exp2f((float)(k - a.k));
             a.k = k;
             a.scale_limit = (uint32_t)__half_as_ushort(__float2half_rn(exp2f((float)(e + 1)))) - 1;

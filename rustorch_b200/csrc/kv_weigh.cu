@@ -16,7 +16,10 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
 constexpr int kBlock = 64;  // query rows in shared memory at a time
-constexpr int kTensorRows = 64;  // rows of a KV head from which kv_weigh_tc.cu's kernel is taken
+// Query rows of a KV head from which kv_weigh_tc.cu's kernel is taken.  8 heads of 16,001 tokens, here and there: D = 128, 32
+// rows 10.4 and 9.5 us, 64 rows 13.1 and 8.7, 128 rows 20.6 and 12.8; D = 64, 32 rows 8.1 and 8.5 (16 x 2000 tokens: 11.9 and
+// 16.2), 64 rows 10.6 and 8.1; D = 256, 32 rows 22.9 and 15.8.
+constexpr int tensor_rows(int head_dim) { return head_dim == 64 ? 64 : 32; }
 
 struct WeighParams {
     const __nv_bfloat16 *q, *k;
@@ -159,7 +162,7 @@ cudaError_t launch_kv_weigh(const void* q, const void* k_cache, const float* lse
     p.n_kv = n_kv, p.group = n_heads / n_kv, p.scale_log2 = scale * kLog2e;
     const int64_t longest = kv_lens ? max_seq : kv_len_uniform;
     if (longest == 0) return cudaSuccess;
-    if (p.group * seq_q >= kTensorRows) {
+    if (p.group * seq_q >= tensor_rows(head_dim) && seq_q > 1) {
         const cudaError_t e = launch_kv_weigh_tc(q, k_cache, lse, weights, batch, n_heads, n_kv, seq_q, head_dim, max_seq, longest, kv_lens,
                                                  kv_len_uniform, scale, stream);
         if (e != cudaErrorNotSupported) return e;
