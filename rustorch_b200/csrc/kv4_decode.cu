@@ -6,6 +6,7 @@
 // byte, two codes c0 + 16 c1: nothing is dequantised.  The scale of K goes onto the 16 x 8 products of a group, that of V, as
 // a product sums over tokens, onto the probabilities of a group's product.
 #include <algorithm>
+#include <atomic>
 
 #include "cache_kernels.h"
 #include "kernels.h"
@@ -432,6 +433,32 @@ __device__ __forceinline__ void fetch(uint32_t to, const LanePlanes& from, int64
     }
 }
 
+// A warp's sums as rows: row(query, dim, four neighbouring dims, sum of p), and once a query total(query, reference, sum of p).
+// They are relative to 2^reference and not yet divided.
+template <int D, class Row, class Total>
+__device__ __forceinline__ void results(const Sums<D>& a, int lane, Row&& row, Total&& total) {
+    using S = Shape<D>;
+    const int g = lane / 4, j = lane % 4;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+        float l = a.l[c];
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(kFullMask, l, off);
+        const float even = exp2f((float)(24 - a.k)), odd = even * 0.0625f;
+#pragma unroll
+        for (int i = 0; i < S::kGroups; ++i) {
+            // the minima's sum of the group is with the lanes 2i + 1
+            const float sum = S::kSpans == 2 ? a.lo[c + 2 * (i / S::kSpanGroups)] : a.lo[c];
+            float y = __shfl_sync(kFullMask, sum, 8 * (i % S::kSpanGroups) + 4 + j);
+            if (S::kSpans == 1) y += __shfl_sync(kFullMask, a.lo2[c + 2], 8 * i + 4 + j);
+            const int d = (i / S::kSpanGroups) * S::R::kSpan + (g >> 1) * (S::R::kSpan / 4) + 8 * (i % S::kSpanGroups) + 4 * (g & 1);
+            row(2 * j + c, d, make_float4(fmaf(a.o[i][0][c], even, y), fmaf(a.o[i][0][c + 2] - a.o[i][0][c], odd, y),
+                                          fmaf(a.o[i][1][c], even, y), fmaf(a.o[i][1][c + 2] - a.o[i][1][c], odd, y)), l);
+        }
+        if (g == 0) total(2 * j + c, a.ref[c], l);
+    }
+}
+
 // A warp is a worker: its run of steps may begin and end inside a (sequence, KV head) and pass over several.  What it has of
 // one that others work on too is a part for the merge kernel: part 2 i of worker i is what its run begins with, 2 i + 1
 // what it ends with.
@@ -442,7 +469,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
     extern __shared__ __align__(16) uint8_t smem[];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, G = p.group, g = lane / 4, j = lane % 4;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, G = p.group;
     const int64_t all = count_steps(p);
     const int workers = (int)min((int64_t)p.workers, all);
     const int worker = warp * gridDim.x + blockIdx.x;  // a launch of few spreads them over the SMs
@@ -514,38 +541,182 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
             if (step0 == 0) p.spans[bh].x = whole ? -1 : 2 * worker + !head;
             if (step0 + steps == n) p.spans[bh].y = worker;
         }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            float l = a.l[c];
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(kFullMask, l, off);
-            const int h_q = 2 * j + c;
-            const bool mine = h_q < G;
-            const float even = exp2f((float)(24 - a.k)), odd = even * 0.0625f, inv = hi > lo ? 1.f / l : 0.f;
-#pragma unroll
-            for (int i = 0; i < S::kGroups; ++i) {
-                // the minima's sum of the group is with the lanes 2i + 1
-                const float sum = S::kSpans == 2 ? a.lo[c + 2 * (i / S::kSpanGroups)] : a.lo[c];
-                float y = __shfl_sync(kFullMask, sum, 8 * (i % S::kSpanGroups) + 4 + j);
-                if (S::kSpans == 1) y += __shfl_sync(kFullMask, a.lo2[c + 2], 8 * i + 4 + j);
-                const int d = (i / S::kSpanGroups) * S::R::kSpan + (g >> 1) * (S::R::kSpan / 4) + 8 * (i % S::kSpanGroups) + 4 * (g & 1);
-                const float4 o = make_float4(fmaf(a.o[i][0][c], even, y), fmaf(a.o[i][0][c + 2] - a.o[i][0][c], odd, y),
-                                             fmaf(a.o[i][1][c], even, y), fmaf(a.o[i][1][c + 2] - a.o[i][1][c], odd, y));
-                if (mine && whole) {
-                    const uint2 packed = make_uint2(float2_to_bf16x2(o.x * inv, o.y * inv), float2_to_bf16x2(o.z * inv, o.w * inv));
-                    *reinterpret_cast<uint2*>(p.out + (bh * G + h_q) * D + d) = packed;
-                } else if (mine) {
+        results<D>(
+            a, lane,
+            [&](int h_q, int d, float4 o, float l) {
+                if (h_q >= G) return;
+                if (!whole) {
                     *reinterpret_cast<float4*>(p.part_o + (part + h_q) * D + d) = o;
+                    return;
                 }
-            }
-            if (mine && g == 0) {
-                if (!whole) p.part_ml[part + h_q] = make_float2(a.ref[c], l);
-                else if (p.lse) p.lse[bh * G + h_q] = hi > lo ? a.ref[c] * kLn2 + logf(l) : -INFINITY;
-            }
-        }
+                const float inv = hi > lo ? 1.f / l : 0.f;
+                *reinterpret_cast<uint2*>(p.out + (bh * G + h_q) * D + d) =
+                    make_uint2(float2_to_bf16x2(o.x * inv, o.y * inv), float2_to_bf16x2(o.z * inv, o.w * inv));
+            },
+            [&](int h_q, float ref, float l) {
+                if (h_q >= G) return;
+                if (!whole) p.part_ml[part + h_q] = make_float2(ref, l);
+                else if (p.lse) p.lse[bh * G + h_q] = hi > lo ? ref * kLn2 + logf(l) : -INFINITY;
+            });
         at += steps;
         if (h == p.n_kv - 1 && step0 + steps == n) first += (int64_t)n * p.n_kv, ++b;
     }
+}
+
+// Short sequences in one launch: a cluster of CTAs is one (sequence, KV head), its warps take the steps in turn, and the
+// results meet in shared memory: the CTA's four warps', then the cluster's CTAs'.  Scores stay there too until the
+// log-sum-exp is known, so that the weights need no launch of their own.  On the device, here and with workers and merge
+// (and weights) launches, 8 heads, D = 128: 1000 tokens 6.0 and 8.4 us (weighed 7.6 and 11.1), 8000 tokens 10.9 and 16.2 (15.8
+// and 19.0), 16,000 tokens 16.4 and 19.4 (24.4 and 21.9); 16 heads, 8000 tokens 13.0 and 15.8 (18.0 and 17.9).  So up to 8
+// steps a warp.
+template <int D>
+struct ClusterShape {
+    using S = Shape<D>;
+    static constexpr int kPitch = D + 4;  // of a query's sums
+    static constexpr int kResults = kWarps * kMaxGroup * kPitch * 4;
+    static size_t smem(int score_steps, int group) { return S::kSmem + kResults + (size_t)score_steps * kWarps * kStep * group * 4; }
+};
+constexpr size_t kHalfSm = 112 * 1024;              // shared memory with which two CTAs fit an SM
+constexpr int kMostCluster = 8, kClusterTurns = 8;  // CTAs of a cluster, steps of a warp in one
+
+__device__ __forceinline__ void cluster_barrier() {
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t remote_address(const void* p, int rank) {  // of what lies at p in CTA `rank`
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return at;
+}
+__device__ __forceinline__ float4 load_remote(const float4* p, int rank) {
+    float4 x;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+                 : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                 : "r"(remote_address(p, rank))
+                 : "memory");
+    return x;
+}
+__device__ __forceinline__ float2 load_remote(const float2* p, int rank) {
+    float2 x;
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(remote_address(p, rank)) : "memory");
+    return x;
+}
+
+// score_steps: steps of a warp at most, where weights are asked for.
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) kv4_cluster_kernel(const DecodeParams p, int score_steps) {
+    using S = Shape<D>;
+    using C = ClusterShape<D>;
+    constexpr int kStages = S::kStages;
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float2 ml[kWarps][kMaxGroup], cta_ml[kMaxGroup];  // reference (-inf: no tokens) and sum of a query's weights
+    __shared__ float lse2[kMaxGroup];
+    float* sums = reinterpret_cast<float*>(smem + S::kSmem);  // [warp][query][kPitch]; the CTA's own in warp 0's place
+    float* scores = reinterpret_cast<float*>(smem + S::kSmem + C::kResults);  // [query][local token]
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int tid = threadIdx.x, lane = tid % 32, warp = tid / 32, G = p.group, ctas = gridDim.x, rank = blockIdx.x;
+    const int64_t b = blockIdx.z, bh = b * p.n_kv + blockIdx.y, rows = bh * p.max_seq;
+    const int len = visible(p, (int)b), steps = (len + kStep - 1) / kStep, every = ctas * kWarps, first = rank * kWarps + warp;
+    uint8_t* ring = smem + warp * kStages * S::kStage;
+    const uint32_t ring_at = (uint32_t)__cvta_generic_to_shared(ring);
+    constexpr int kPiece = S::kScaleRow < 16 ? S::kScaleRow : 16;
+    const LanePlanes planes{p.k_codes + lane * 16, p.v_codes + lane * 4, p.k_scales + lane * kPiece, p.v_scales + lane * kPiece};
+    auto prefetch = [&](int s, int slot) {
+        const int valid = len - s * kStep;
+        const uint32_t to = ring_at + slot * S::kStage;
+        if (valid >= kStep) fetch<D>(to, planes, rows + s * kStep, kStep, lane);
+        else if (valid > 0) fetch<D>(to, planes, rows + s * kStep, valid, lane);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i)
+        if (first + (int64_t)i * every < steps) prefetch(first + i * every, i);
+        else asm volatile("cp.async.commit_group;" ::: "memory");
+    Queries<D> q;
+    q.load(p, bh, lane);
+    Sums<D> a = {};
+    a.top[0] = a.top[1] = -INFINITY;
+    int slot = 0, turn = 0;
+    const int local = score_steps * kWarps * kStep;  // tokens of a query's scores
+    for (int s = first; s < steps; s += every, ++turn) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+        __syncwarp();
+        int next = slot + kStages - 1;
+        if (next >= kStages) next -= kStages;
+        prefetch(s + (kStages - 1) * every, next);
+        step<D>(ring + slot * S::kStage, len - s * kStep, q, a, lane, score_steps ? scores + (turn * kWarps + warp) * kStep : nullptr, local, G);
+        if (++slot == kStages) slot = 0;
+    }
+    const bool any = first < steps;
+    results<D>(
+        a, lane,
+        [&](int h, int d, float4 o, float) {
+            if (h < G) *reinterpret_cast<float4*>(sums + (warp * kMaxGroup + h) * C::kPitch + d) = o;
+        },
+        [&](int h, float ref, float l) { ml[warp][h] = make_float2(any ? ref : -INFINITY, l); });
+    __syncthreads();
+    // ---- the CTA's: a thread keeps to its places, so that warp 0's can be overwritten
+    for (int i = tid; i < G * (D / 4); i += kThreads) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4;
+        float m = -INFINITY, l = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, ml[w][h].x);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float2 x = ml[w][h];
+            if (x.x == -INFINITY) continue;
+            const float f = exp2f(x.x - m);
+            const float4 y = *reinterpret_cast<const float4*>(sums + (w * kMaxGroup + h) * C::kPitch + d);
+            o.x = fmaf(y.x, f, o.x), o.y = fmaf(y.y, f, o.y), o.z = fmaf(y.z, f, o.z), o.w = fmaf(y.w, f, o.w);
+            l = fmaf(x.y, f, l);
+        }
+        *reinterpret_cast<float4*>(sums + h * C::kPitch + d) = o;
+        if (d == 0) cta_ml[h] = make_float2(m, l);
+    }
+    cluster_barrier();
+    // ---- the cluster's: each CTA a share of the places
+    auto total_of = [&](int h, float& m, float& l) {
+        m = -INFINITY, l = 0.f;
+        for (int r = 0; r < ctas; ++r) m = fmaxf(m, load_remote(&cta_ml[h], r).x);
+        for (int r = 0; r < ctas; ++r) {
+            const float2 x = load_remote(&cta_ml[h], r);
+            if (x.x != -INFINITY) l = fmaf(x.y, exp2f(x.x - m), l);
+        }
+    };
+    for (int i = rank * kThreads + tid; i < G * (D / 4); i += ctas * kThreads) {
+        const int h = i / (D / 4), d = i % (D / 4) * 4;
+        float m, l;
+        total_of(h, m, l);
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int r = 0; r < ctas; ++r) {
+            const float2 x = load_remote(&cta_ml[h], r);
+            const float4 y = load_remote(reinterpret_cast<const float4*>(sums + h * C::kPitch + d), r);
+            const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - m);
+            o.x = fmaf(y.x, f, o.x), o.y = fmaf(y.y, f, o.y), o.z = fmaf(y.z, f, o.z), o.w = fmaf(y.w, f, o.w);
+        }
+        const float inv = len > 0 ? 1.f / l : 0.f;
+        *reinterpret_cast<uint2*>(p.out + (bh * G + h) * D + d) =
+            make_uint2(float2_to_bf16x2(o.x * inv, o.y * inv), float2_to_bf16x2(o.z * inv, o.w * inv));
+        if (d == 0 && p.lse) p.lse[bh * G + h] = len > 0 ? m * kLn2 + logf(l) : -INFINITY;
+    }
+    if (score_steps) {
+        if (tid < G) {
+            float m, l;
+            total_of(tid, m, l);
+            lse2[tid] = m + log2f(l);
+        }
+        __syncthreads();
+        for (int i = tid; i < local; i += kThreads) {
+            const int64_t t = ((int64_t)first - warp + i / (kWarps * kStep) * every) * kStep + i % (kWarps * kStep);
+            if (t >= len) break;  // the later ones are further on
+            float w = 0.f;
+            for (int h = 0; h < G; ++h) w += exp2f(scores[h * local + i] - lse2[h]);
+            p.weights[rows + t] += w;
+        }
+    }
+    cluster_barrier();  // nobody leaves while its shared memory is read
 }
 
 constexpr int kMergeWarps = 8, kMergeParts = 256;
@@ -664,6 +835,49 @@ __global__ void __launch_bounds__(kThreads) kv4_weights_kernel(const DecodeParam
     }
 }
 
+// Clusters of `size` CTAs with that much shared memory that the device has resident at a time, asked for once.
+template <int D>
+cudaError_t cluster_slots(int size, size_t smem, int& slots) {
+    static std::atomic<int> known[64][4][2];  // [device][log2 size][shared memory: up to half of an SM's, or more]
+    int dev = 0;
+    const cudaError_t at = cudaGetDevice(&dev);
+    if (at != cudaSuccess) return at;
+    const int log2 = size == 8 ? 3 : size == 4 ? 2 : 1, large = smem > kHalfSm;
+    std::atomic<int>* entry = dev < 64 ? &known[dev][log2][large] : nullptr;
+    if (entry && (slots = entry->load(std::memory_order_relaxed)) > 0) return cudaSuccess;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(size, 1024);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = large ? ClusterShape<D>::smem(kClusterTurns, kMaxGroup) : kHalfSm;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = size, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&slots, kv4_cluster_kernel<D>, &cfg);
+    if (e == cudaSuccess && entry) entry->store(std::max(slots, 1), std::memory_order_relaxed);
+    return e;
+}
+
+// The largest cluster that all groups can have at once and whose warps have a step each at least; 0: none, or too many steps.
+template <int D>
+cudaError_t pick_cluster(int64_t groups, int64_t steps, bool weighed, int group, int& cluster, int& turns, size_t& smem) {
+    const cudaError_t at = set_max_dynamic_smem_once<kv4_cluster_kernel<D>>((int)std::max(ClusterShape<D>::smem(kClusterTurns, kMaxGroup), kHalfSm));
+    if (at != cudaSuccess) return at;
+    for (cluster = kMostCluster; cluster > 1; cluster /= 2) {
+        turns = (int)((steps + cluster * kWarps - 1) / (cluster * kWarps));
+        if (turns > kClusterTurns) break;  // smaller clusters have more
+        if (steps < cluster * kWarps) continue;
+        smem = ClusterShape<D>::smem(weighed ? turns : 0, group);
+        int slots = 0;
+        const cudaError_t e = cluster_slots<D>(cluster, smem, slots);
+        if (e != cudaSuccess) return e;
+        if (groups <= slots) return cudaSuccess;
+    }
+    cluster = 0;
+    return cudaSuccess;
+}
+
 // Workers of a launch: as many warps as fit at a time, or one for every step.
 int workers_of(int64_t batch, int n_kv, int head_dim, int64_t max_seq) {
     const int per_sm = kWarps * (head_dim == 64 ? Shape<64>::kPerSm : head_dim == 128 ? Shape<128>::kPerSm : Shape<256>::kPerSm);
@@ -703,6 +917,32 @@ cudaError_t launch_kv4_decode(const Kv4Cache& c, const void* q, void* out, float
         p.scores = (float*)ws;
     }
     p.lse = lse;
+    // One launch where all clusters are resident at once and a warp has few steps.
+    const int64_t groups = batch * n_kv, longest = kv_lens ? max_seq : kv_len_uniform, steps = (longest + kStep - 1) / kStep;
+    if (steps <= (int64_t)kMostCluster * kWarps * kClusterTurns && groups <= sm_count() / 2) {
+        int cluster = 0, turns = 0;
+        size_t smem = 0;
+        const cudaError_t e = for_head_dim(head_dim, [&](auto d) {
+            return pick_cluster<decltype(d)::value>(groups, steps, weights != nullptr, p.group, cluster, turns, smem);
+        });
+        if (e != cudaSuccess) return e;
+        if (cluster) return for_head_dim(head_dim, [&](auto d) {
+            constexpr int D = decltype(d)::value;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(cluster, n_kv, (unsigned)batch);
+            cfg.blockDim = dim3(kThreads);
+            cfg.dynamicSmemBytes = smem;
+            cfg.stream = stream;
+            cudaLaunchAttribute attr[2];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+            attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attr[1].val.programmaticStreamSerializationAllowed = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = 2;
+            return cudaLaunchKernelEx(&cfg, kv4_cluster_kernel<D>, p, weights ? turns : 0);
+        });
+    }
     return for_head_dim(head_dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
         cudaError_t e = set_max_dynamic_smem_once<kv4_decode_kernel<D>>(Shape<D>::kSmem);
