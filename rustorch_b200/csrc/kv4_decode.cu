@@ -741,12 +741,24 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_merge_kernel(const Decod
 #pragma unroll
     for (int off = 16; off; off >>= 1) m = fmaxf(m, __shfl_xor_sync(kFullMask, m, off));
     float o[kPer] = {}, l = 0.f;
-    auto add = [&](int r, float f) {
-        const float* from = p.part_o + part(r) * D + lane * kPer;
+    // `count` rows from part r on, every `every`-th, times their factors: the loads of a batch are in flight at once
+    constexpr int kBatch = 16 / (kPer / 2);
+    auto add = [&](int r, int count, int every, auto&& factor_of) {
+        for (int k0 = 0; k0 < count; k0 += kBatch) {
+            float2 v[kBatch][kPer / 2];
 #pragma unroll
-        for (int k = 0; k < kPer; k += 2) {
-            const float2 v = *reinterpret_cast<const float2*>(from + k);
-            o[k] = fmaf(v.x, f, o[k]), o[k + 1] = fmaf(v.y, f, o[k + 1]);
+            for (int u = 0; u < kBatch; ++u) {
+                const float* from = p.part_o + part(r + min(k0 + u, count - 1) * every) * D + lane * kPer;
+#pragma unroll
+                for (int k = 0; k < kPer / 2; ++k) v[u][k] = *reinterpret_cast<const float2*>(from + 2 * k);
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                if (k0 + u >= count) break;
+                const float f = factor_of(r + (k0 + u) * every);
+#pragma unroll
+                for (int k = 0; k < kPer / 2; ++k) o[2 * k] = fmaf(v[u][k].x, f, o[2 * k]), o[2 * k + 1] = fmaf(v[u][k].y, f, o[2 * k + 1]);
+            }
         }
     };
     if constexpr (kWide) {
@@ -765,8 +777,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_merge_kernel(const Decod
                 l += x.y * f;
             }
             __syncthreads();
-#pragma unroll 8
-            for (int r = warp; r < count; r += kMergeWarps) add(r0 + r, factor[r]);
+            if (warp < count)
+                add(r0 + warp, (count - warp + kMergeWarps - 1) / kMergeWarps, kMergeWarps, [&](int r) { return factor[r - r0]; });
         }
 #pragma unroll
         for (int off = 16; off; off >>= 1) l += __shfl_xor_sync(kFullMask, l, off);
@@ -784,13 +796,18 @@ __global__ void __launch_bounds__(32 * kMergeWarps) kv4_merge_kernel(const Decod
             p.out[(int64_t)row * D + threadIdx.x] = __float2bfloat16(v / l);
         }
     } else {
-#pragma unroll 4
-        for (int r = 0; r < n; ++r) {
-            const float2 x = p.part_ml[part(r)];
-            const float f = exp2f(x.x - m);
-            l += x.y * f;
-            add(r, f);
+        for (int r0 = 0; r0 < n; r0 += 32) {  // a factor a lane
+            const int count = min(32, n - r0);
+            float f = 0.f;
+            if (lane < count) {
+                const float2 x = p.part_ml[part(r0 + lane)];
+                f = exp2f(x.x - m);
+                l = fmaf(x.y, f, l);
+            }
+            add(r0, count, 1, [&](int r) { return __shfl_sync(kFullMask, f, r - r0); });
         }
+#pragma unroll
+        for (int off = 16; off; off >>= 1) l += __shfl_xor_sync(kFullMask, l, off);
 #pragma unroll
         for (int k = 0; k < kPer; k += 2)
             *reinterpret_cast<uint32_t*>(p.out + (int64_t)row * D + kPer * lane + k) = float2_to_bf16x2(o[k] / l, o[k + 1] / l);
