@@ -54,9 +54,8 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // A code is the IEEE quotient (x - lo) / scale rounded to a whole number.  It is first taken from a product with 1 / scale,
 // which is within 2^-18 of it; only an octet in which that leaves a value in doubt (within 2^-15 of the middle between two
 // codes, or outside 0 to 15) takes the quotient itself and clamps it.  10,194 tokens of 8 heads, D = 128, with their
-// read-back: 80.6 us with all values divided, 37.3 with a reciprocal and each value clamped (460 instructions for two rows,
-// which bounded it), 31 with pairs of values and the rare cases apart (288; 20.8 us of it here, 2.6 TB/s: half of the
-// time is now the latency of the loads and of few blocks).
+// read-back: 80.6 us with all values divided, 37.3 with a reciprocal and each value clamped (29 instructions a value at 0.74
+// of the issue rate), 31 with pairs of values and the rare cases apart (18 a value; 20.8 us of it here, 2.6 TB/s).
 template <int D>
 __device__ __forceinline__ uint32_t quantise_octet(uint4 raw, uint32_t& scale_word) {
     using R = Kv4Row<D>;

@@ -263,8 +263,7 @@ cudaError_t launch_kv_evict(const EvictPlanes& planes, const float* weights, flo
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
-    // Not chained to the kernel ahead: CTAs that became resident beside the last ones of that kernel crowded a few SMs (8 heads
-    // of 30,001 tokens, calls back to back: 37 us a call chained, 29 not).
+    // Not chained to the kernel ahead (8 heads of 30,001 tokens, calls back to back: 37 us a call chained, 29 not).
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;

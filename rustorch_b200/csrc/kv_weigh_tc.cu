@@ -3,12 +3,15 @@
 //
 // A CTA takes every so many-th tile of 128 tokens of a (sequence, KV head).  A tile's keys are the A operand, blocks of 64
 // query rows pass by as B through a ring of four, and the 128 x 64 scores through four TMEM buffers: what is queued there
-// covers the load of the next tile's keys and the latency of the rows' loads (with rings of two that was 24 us of the case below).  A token is a TMEM lane, so a thread of the four epilogue warps has a token's
-// scores to itself: it adds up their exponentials in a register, with the rows' log-sum-exps broadcast from shared memory,
+// covers the load of the next tile's keys and the latency of the rows' loads (worth little by itself: 64 queries on 16,001
+// tokens, 32 heads on 8, D = 128, took 24.3 us with rings of two and 24.1 with these; the mask's test compiled apart from
+// the blocks without one brought 21.7).  A token is a TMEM lane, so a thread of the four epilogue warps has a token's scores
+// to itself: it adds up their exponentials in a register, with the rows' log-sum-exps broadcast from shared memory,
 // and writes the token's weight once.  One thread issues all loads and products.  Two CTAs an SM.
 //
-// What bounds it: the exponentials, 16 a clock and SM (512 clocks a block, of which the products take 150).  They are ex2's,
-// not a short polynomial's, since the weights are f32 sums.
+// What bounds it: no pipe is full.  The exponentials come nearest, 16 a clock and SM (512 clocks a block): that pipe is busy
+// for 40 % of the active clocks, and stalls are fixed latency, TMEM reads, shared memory and barriers, in this order.  They are
+// ex2's, not a short polynomial's, since the weights are f32 sums.
 #include "cache_kernels.h"
 #include "kernels.h"
 #include "tc_ptx.cuh"
