@@ -9,6 +9,7 @@
 #include <atomic>
 
 #include "cache_kernels.h"
+#include "cluster.cuh"
 #include "kernels.h"
 #include "kv4.cuh"
 
@@ -578,29 +579,6 @@ struct ClusterShape {
 };
 constexpr size_t kHalfSm = 112 * 1024;              // shared memory with which two CTAs fit an SM
 constexpr int kMostCluster = 8, kClusterTurns = 8;  // CTAs of a cluster, steps of a warp in one
-
-__device__ __forceinline__ void cluster_barrier() {
-    __syncwarp();
-    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
-}
-__device__ __forceinline__ uint32_t remote_address(const void* p, int rank) {  // of what lies at p in CTA `rank`
-    uint32_t at;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    return at;
-}
-__device__ __forceinline__ float4 load_remote(const float4* p, int rank) {
-    float4 x;
-    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-                 : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
-                 : "r"(remote_address(p, rank))
-                 : "memory");
-    return x;
-}
-__device__ __forceinline__ float2 load_remote(const float2* p, int rank) {
-    float2 x;
-    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(remote_address(p, rank)) : "memory");
-    return x;
-}
 
 // score_steps: steps of a warp at most, where weights are asked for.
 template <int D>

@@ -8,6 +8,7 @@
 #include <algorithm>
 
 #include "cache_kernels.h"
+#include "cluster.cuh"
 #include "kernels.h"
 #include "common.cuh"
 
@@ -33,29 +34,6 @@ struct SelectShared {
     uint64_t warps[kWarps];
     uint32_t digit, above;
 };
-
-__device__ __forceinline__ void cluster_barrier() {
-    asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;" ::: "memory");
-}
-// What lies at `p` in the shared memory of the cluster's CTA `rank`.
-__device__ __forceinline__ uint32_t remote_address(const void* p, int rank) {
-    uint32_t at;
-    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-    return at;
-}
-__device__ __forceinline__ uint32_t load_remote(const uint32_t* p, int rank) {
-    uint32_t x;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(x) : "r"(remote_address(p, rank)) : "memory");
-    return x;
-}
-__device__ __forceinline__ uint4 load_remote4(const uint32_t* p, int rank) {
-    uint4 x;
-    asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];"
-                 : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
-                 : "r"(remote_address(p, rank))
-                 : "memory");
-    return x;
-}
 
 // A key that orders floats as unsigned integers, -0 as 0 and every NaN above infinity.
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -110,7 +88,7 @@ __device__ __forceinline__ void choose(SelectShared& sh, int C, int rank, int co
         const int low = kBins - 4 - 4 * tid;
         uint4 u = *reinterpret_cast<const uint4*>(&bins[low]);
         for (int r = 1; r < C; ++r) {
-            const uint4 x = load_remote4(&bins[low], rank + r < C ? rank + r : rank + r - C);
+            const uint4 x = load_remote(reinterpret_cast<const uint4*>(&bins[low]), rank + r < C ? rank + r : rank + r - C);
             u.x += x.x, u.y += x.y, u.z += x.z, u.w += x.w;
         }
         const uint32_t all = u.x + u.y + u.z + u.w;
