@@ -5,6 +5,13 @@
 // A code in the low bits of a 16-bit half is the f16 subnormal code * 2^-24, which mma.sync multiplies exactly, and so is a
 // byte, two codes c0 + 16 c1: nothing is dequantised.  The scale of K goes onto the 16 x 8 products of a group, that of V, as
 // a product sums over tokens, onto the probabilities of a group's product.
+//
+// A probability has f16's 11 bits, its product with a scale 22: it is used in two f16 parts.  One part alone is off by what
+// sum(p scale code) and sum(p lo) do not share, and each of these is several times the values' size and cancels the other:
+// where scores are nearly equal (a spread of 0.0003 in log2, 20,000 tokens, N(0, 1) values) the result was off by 1.8 %, and
+// is by 0.2 now, bf16's own rounding.  A KV head of up to four queries has them twice in the products' eight columns, the
+// second time with the second part; with more queries the second part takes products of its own.  64 sequences of 1024 to
+// 8192 tokens, 32 heads on 8, D = 128: 84.7 us with one part, 87.9 with two by columns, 90.6 with products.
 #include <algorithm>
 #include <atomic>
 
@@ -110,6 +117,10 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
     const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ uint32_t rest_half2(uint32_t a, uint32_t b, uint32_t ab) {  // a b - ab
+    const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), __hneg2(*reinterpret_cast<const __half2*>(&ab)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
 __device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
     const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -140,7 +151,7 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[kWords], const uint8_t*
 }
 
 // One (sequence, KV head)'s queries as the B operand of the score products: lane (g, j) = (lane / 4, lane % 4) holds query
-// g's octets of quarter j.  The queries are scaled by a power of two that brings their largest value to 2^14, where
+// g's octets of quarter j; with kTwice, queries 0 to 3 again as 4 to 7.  The queries are scaled by a power of two that brings their largest value to 2^14, where
 // bf16's 8 bits fit f16 exactly (values 2^-31 of the largest and smaller lose bits).
 template <int D>
 struct Queries {
@@ -148,9 +159,10 @@ struct Queries {
     uint32_t sums[Shape<D>::kSpans];     // lane j's group of a span: its sum / 64 in two f16 parts, 22 bits
     float factor[2];                     // scale_log2 * 2^24 / the power of two, of queries 2j and 2j + 1
 
+    template <bool kTwice>
     __device__ __forceinline__ void load(const DecodeParams& p, int64_t bh, int lane) {
         using S = Shape<D>;
-        const int g = lane / 4, j = lane % 4;
+        const int g = kTwice ? lane / 4 % 4 : lane / 4, j = lane % 4;
         uint4 raw[S::kGroups];
         float top = 0.f;
         bool nan = false;
@@ -205,7 +217,8 @@ struct Queries {
     }
 };
 
-// What a warp has summed so far.  Lane (g, j) holds queries 2j and 2j + 1.
+// What a warp has summed so far.  Lane (g, j) holds queries 2j and 2j + 1.  With kTwice the lanes j < 2 hold the sums of the
+// products' first parts and j + 2 those of the second ones in `o`; all else is the same in both.
 template <int D>
 struct Sums {
     float o[D / 32][2][4];       // [group][0-1, 2-3 of a lane's four dims]: sum p scale c 2^(k - 24), {q 2j, 2j+1} x {c0, c0 + 16 c1}
@@ -224,7 +237,7 @@ __device__ __forceinline__ void load_transposed(uint32_t (&r)[4], uint32_t at) {
 }
 
 // 32 tokens (valid of them) that lie in shared memory.  scores: [query][max_seq] from this step's first token on, or null.
-template <int D>
+template <int D, bool kTwice>
 __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Queries<D>& q, Sums<D>& a, int lane, float* scores,
                                      int64_t max_seq, int group) {
     using S = Shape<D>;
@@ -346,6 +359,7 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
         prob[tb][1] = transposed(pack_half2(e[2], e[3]));
     }
     const uint32_t up = power_half2(a.k);
+    const uint32_t rest = kTwice && g < 4 ? 0u : 0xffffffffu;  // 0: this lane's column takes the first parts
     // V and its scales come transposed: 16-bit unit g of a row (4 codes of a group, or a scale or minimum) to the lanes g, those
     // of tokens 2j and 2j + 1 in one register.
     const uint32_t v_at = (uint32_t)__cvta_generic_to_shared(vc) + (lane & 15) * S::kVPitch + (lane >> 4) * 16;
@@ -381,12 +395,18 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int s = (gi + c) / S::kSpanGroups, from = 8 * ((gi + c) % S::kSpanGroups) + j;
-                const uint32_t b0 = mul_half2(prob[tb][0], __shfl_sync(kFullMask, f[tb][0][s], from)),
-                               b1 = mul_half2(prob[tb][1], __shfl_sync(kFullMask, f[tb][1][s], from));
-                uint32_t u0 = w[2 * c], u1 = w[2 * c + 1];
+                const uint32_t f0 = __shfl_sync(kFullMask, f[tb][0][s], from), f1 = __shfl_sync(kFullMask, f[tb][1][s], from);
+                uint32_t b0 = mul_half2(prob[tb][0], f0), b1 = mul_half2(prob[tb][1], f1);
+                // what they were rounded by (exact), or, of a column with the first parts, themselves
+                const uint32_t r0 = rest_half2(prob[tb][0], f0, b0 & rest), r1 = rest_half2(prob[tb][1], f1, b1 & rest);
+                if (kTwice) b0 = r0, b1 = r1;
+                const uint32_t u0 = w[2 * c], u1 = w[2 * c + 1], x0 = __byte_perm(u0, 0, 0x4341), x1 = __byte_perm(u1, 0, 0x4341);
                 mma_f16(a.o[gi + c][0], u0 & 0x000f000fu, u0 & 0x00ff00ffu, u1 & 0x000f000fu, u1 & 0x00ff00ffu, b0, b1);
-                u0 = __byte_perm(u0, 0, 0x4341), u1 = __byte_perm(u1, 0, 0x4341);
-                mma_f16(a.o[gi + c][1], u0 & 0x000f000fu, u0, u1 & 0x000f000fu, u1, b0, b1);
+                mma_f16(a.o[gi + c][1], x0 & 0x000f000fu, x0, x1 & 0x000f000fu, x1, b0, b1);
+                if (!kTwice) {
+                    mma_f16(a.o[gi + c][0], u0 & 0x000f000fu, u0 & 0x00ff00ffu, u1 & 0x000f000fu, u1 & 0x00ff00ffu, r0, r1);
+                    mma_f16(a.o[gi + c][1], x0 & 0x000f000fu, x0, x1 & 0x000f000fu, x1, r0, r1);
+                }
             }
         }
     }
@@ -436,7 +456,7 @@ __device__ __forceinline__ void fetch(uint32_t to, const LanePlanes& from, int64
 
 // A warp's sums as rows: row(query, dim, four neighbouring dims, sum of p), and once a query total(query, reference, sum of p).
 // They are relative to 2^reference and not yet divided.
-template <int D, class Row, class Total>
+template <int D, bool kTwice, class Row, class Total>
 __device__ __forceinline__ void results(const Sums<D>& a, int lane, Row&& row, Total&& total) {
     using S = Shape<D>;
     const int g = lane / 4, j = lane % 4;
@@ -453,8 +473,13 @@ __device__ __forceinline__ void results(const Sums<D>& a, int lane, Row&& row, T
             float y = __shfl_sync(kFullMask, sum, 8 * (i % S::kSpanGroups) + 4 + j);
             if (S::kSpans == 1) y += __shfl_sync(kFullMask, a.lo2[c + 2], 8 * i + 4 + j);
             const int d = (i / S::kSpanGroups) * S::R::kSpan + (g >> 1) * (S::R::kSpan / 4) + 8 * (i % S::kSpanGroups) + 4 * (g & 1);
-            row(2 * j + c, d, make_float4(fmaf(a.o[i][0][c], even, y), fmaf(a.o[i][0][c + 2] - a.o[i][0][c], odd, y),
-                                          fmaf(a.o[i][1][c], even, y), fmaf(a.o[i][1][c + 2] - a.o[i][1][c], odd, y)), l);
+            float o[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                o[k] = a.o[i][k / 2][c + k % 2 * 2];
+                if (kTwice) o[k] += __shfl_xor_sync(kFullMask, o[k], 2);
+            }
+            row(2 * j + c, d, make_float4(fmaf(o[0], even, y), fmaf(o[1] - o[0], odd, y), fmaf(o[2], even, y), fmaf(o[3] - o[2], odd, y)), l);
         }
         if (g == 0) total(2 * j + c, a.ref[c], l);
     }
@@ -463,7 +488,7 @@ __device__ __forceinline__ void results(const Sums<D>& a, int lane, Row&& row, T
 // A warp is a worker: its run of steps may begin and end inside a (sequence, KV head) and pass over several.  What it has of
 // one that others work on too is a part for the merge kernel: part 2 i of worker i is what its run begins with, 2 i + 1
 // what it ends with.
-template <int D>
+template <int D, bool kTwice>
 __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(const DecodeParams p) {
     using S = Shape<D>;
     constexpr int kStages = S::kStages;
@@ -522,7 +547,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
 #pragma unroll
         for (int i = 0; i < kStages - 1; ++i) prefetch(i, i);
         Queries<D> q;
-        q.load(p, bh, lane);
+        q.template load<kTwice>(p, bh, lane);
         Sums<D> a = {};
         a.top[0] = a.top[1] = -INFINITY;
         int slot = 0;
@@ -532,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
             int next = slot + kStages - 1;
             if (next >= kStages) next -= kStages;
             prefetch(s + kStages - 1, next);
-            step<D>(ring + slot * S::kStage, hi - t0, q, a, lane, p.scores ? p.scores + rows * G + t0 : nullptr, p.max_seq, G);
+            step<D, kTwice>(ring + slot * S::kStage, hi - t0, q, a, lane, p.scores ? p.scores + rows * G + t0 : nullptr, p.max_seq, G);
             if (++slot == kStages) slot = 0;
         }
         // ---- the result, or a part of it
@@ -542,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
             if (step0 == 0) p.spans[bh].x = whole ? -1 : 2 * worker + !head;
             if (step0 + steps == n) p.spans[bh].y = worker;
         }
-        results<D>(
+        results<D, kTwice>(
             a, lane,
             [&](int h_q, int d, float4 o, float l) {
                 if (h_q >= G) return;
@@ -581,7 +606,7 @@ constexpr size_t kHalfSm = 112 * 1024;              // shared memory with which 
 constexpr int kMostCluster = 8, kClusterTurns = 8;  // CTAs of a cluster, steps of a warp in one
 
 // score_steps: steps of a warp at most, where weights are asked for.
-template <int D>
+template <int D, bool kTwice>
 __global__ void __launch_bounds__(kThreads, 1) kv4_cluster_kernel(const DecodeParams p, int score_steps) {
     using S = Shape<D>;
     using C = ClusterShape<D>;
@@ -612,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_cluster_kernel(const DecodePa
         if (first + (int64_t)i * every < steps) prefetch(first + i * every, i);
         else asm volatile("cp.async.commit_group;" ::: "memory");
     Queries<D> q;
-    q.load(p, bh, lane);
+    q.template load<kTwice>(p, bh, lane);
     Sums<D> a = {};
     a.top[0] = a.top[1] = -INFINITY;
     int slot = 0, turn = 0;
@@ -623,11 +648,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_cluster_kernel(const DecodePa
         int next = slot + kStages - 1;
         if (next >= kStages) next -= kStages;
         prefetch(s + (kStages - 1) * every, next);
-        step<D>(ring + slot * S::kStage, len - s * kStep, q, a, lane, score_steps ? scores + (turn * kWarps + warp) * kStep : nullptr, local, G);
+        step<D, kTwice>(ring + slot * S::kStage, len - s * kStep, q, a, lane, score_steps ? scores + (turn * kWarps + warp) * kStep : nullptr, local, G);
         if (++slot == kStages) slot = 0;
     }
     const bool any = first < steps;
-    results<D>(
+    results<D, kTwice>(
         a, lane,
         [&](int h, int d, float4 o, float) {
             if (h < G) *reinterpret_cast<float4*>(sums + (warp * kMaxGroup + h) * C::kPitch + d) = o;
@@ -830,8 +855,14 @@ __global__ void __launch_bounds__(kThreads) kv4_weights_kernel(const DecodeParam
     }
 }
 
+// f(head dim, whether a KV head's queries fit an operand twice)
+template <class F>
+cudaError_t for_form(int head_dim, int group, F&& f) {
+    return for_head_dim(head_dim, [&](auto d) { return group <= 4 ? f(d, std::true_type{}) : f(d, std::false_type{}); });
+}
+
 // Clusters of `size` CTAs with that much shared memory that the device has resident at a time, asked for once.
-template <int D>
+template <int D, bool kTwice>
 cudaError_t cluster_slots(int size, size_t smem, int& slots) {
     static std::atomic<int> known[64][4][2];  // [device][log2 size][shared memory: up to half of an SM's, or more]
     int dev = 0;
@@ -849,15 +880,15 @@ cudaError_t cluster_slots(int size, size_t smem, int& slots) {
     attr[0].val.clusterDim.x = size, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaOccupancyMaxActiveClusters(&slots, kv4_cluster_kernel<D>, &cfg);
+    const cudaError_t e = cudaOccupancyMaxActiveClusters(&slots, kv4_cluster_kernel<D, kTwice>, &cfg);
     if (e == cudaSuccess && entry) entry->store(std::max(slots, 1), std::memory_order_relaxed);
     return e;
 }
 
 // The largest cluster that all groups can have at once and whose warps have a step each at least; 0: none, or too many steps.
-template <int D>
+template <int D, bool kTwice>
 cudaError_t pick_cluster(int64_t groups, int64_t steps, bool weighed, int group, int& cluster, int& turns, size_t& smem) {
-    const cudaError_t at = set_max_dynamic_smem_once<kv4_cluster_kernel<D>>((int)std::max(ClusterShape<D>::smem(kClusterTurns, kMaxGroup), kHalfSm));
+    const cudaError_t at = set_max_dynamic_smem_once<kv4_cluster_kernel<D, kTwice>>((int)std::max(ClusterShape<D>::smem(kClusterTurns, kMaxGroup), kHalfSm));
     if (at != cudaSuccess) return at;
     for (cluster = kMostCluster; cluster > 1; cluster /= 2) {
         turns = (int)((steps + cluster * kWarps - 1) / (cluster * kWarps));
@@ -865,7 +896,7 @@ cudaError_t pick_cluster(int64_t groups, int64_t steps, bool weighed, int group,
         if (steps < cluster * kWarps) continue;
         smem = ClusterShape<D>::smem(weighed ? turns : 0, group);
         int slots = 0;
-        const cudaError_t e = cluster_slots<D>(cluster, smem, slots);
+        const cudaError_t e = cluster_slots<D, kTwice>(cluster, smem, slots);
         if (e != cudaSuccess) return e;
         if (groups <= slots) return cudaSuccess;
     }
@@ -917,12 +948,13 @@ cudaError_t launch_kv4_decode(const Kv4Cache& c, const void* q, void* out, float
     if (steps <= (int64_t)kMostCluster * kWarps * kClusterTurns && groups <= sm_count() / 2) {
         int cluster = 0, turns = 0;
         size_t smem = 0;
-        const cudaError_t e = for_head_dim(head_dim, [&](auto d) {
-            return pick_cluster<decltype(d)::value>(groups, steps, weights != nullptr, p.group, cluster, turns, smem);
+        const cudaError_t e = for_form(head_dim, p.group, [&](auto d, auto t) {
+            return pick_cluster<decltype(d)::value, decltype(t)::value>(groups, steps, weights != nullptr, p.group, cluster, turns, smem);
         });
         if (e != cudaSuccess) return e;
-        if (cluster) return for_head_dim(head_dim, [&](auto d) {
+        if (cluster) return for_form(head_dim, p.group, [&](auto d, auto t) {
             constexpr int D = decltype(d)::value;
+            constexpr bool kTwice = decltype(t)::value;
             cudaLaunchConfig_t cfg = {};
             cfg.gridDim = dim3(cluster, n_kv, (unsigned)batch);
             cfg.blockDim = dim3(kThreads);
@@ -935,14 +967,15 @@ cudaError_t launch_kv4_decode(const Kv4Cache& c, const void* q, void* out, float
             attr[1].val.programmaticStreamSerializationAllowed = 1;
             cfg.attrs = attr;
             cfg.numAttrs = 2;
-            return cudaLaunchKernelEx(&cfg, kv4_cluster_kernel<D>, p, weights ? turns : 0);
+            return cudaLaunchKernelEx(&cfg, kv4_cluster_kernel<D, kTwice>, p, weights ? turns : 0);
         });
     }
-    return for_head_dim(head_dim, [&](auto d) {
+    return for_form(head_dim, p.group, [&](auto d, auto t) {
         constexpr int D = decltype(d)::value;
-        cudaError_t e = set_max_dynamic_smem_once<kv4_decode_kernel<D>>(Shape<D>::kSmem);
+        constexpr bool kTwice = decltype(t)::value;
+        cudaError_t e = set_max_dynamic_smem_once<kv4_decode_kernel<D, kTwice>>(Shape<D>::kSmem);
         if (e != cudaSuccess) return e;
-        e = launch_chained(kv4_decode_kernel<D>, dim3((p.workers + kWarps - 1) / kWarps), kThreads, Shape<D>::kSmem, stream, p);
+        e = launch_chained(kv4_decode_kernel<D, kTwice>, dim3((p.workers + kWarps - 1) / kWarps), kThreads, Shape<D>::kSmem, stream, p);
         if (e == cudaSuccess && p.workers > 1) {
             // a row has about workers * group / rows parts
             const int64_t n = batch * n_heads;

@@ -1,0 +1,52 @@
+"""Calls of the 4-bit cache and of eviction next to the edges of what their documentation allows, against forms in 64 bits."""
+import math
+
+import pytest
+
+from tests import kv4_plain as plain
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture
+def rt():
+    import rustorch_b200 as rt
+    return rt
+
+
+def _i32(*v):
+    return torch.tensor(v, dtype=torch.int32, device="cuda")
+
+
+def _randn(*shape, seed=0, scale=1.0):
+    return (torch.randn(shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)) * scale).bfloat16()
+
+
+def _cut(cache, n):
+    return type(cache)(*(t[:, :, :n].contiguous() for t in cache))
+
+
+# ------------------------------------------------------------------------------------------------ decode
+
+
+# max_seq 8192 is the longest that one launch of clusters takes; 20,000 is cut into runs for the workers
+@pytest.mark.parametrize("S,n", [(8192, 8192), (20000, 20000)])
+@pytest.mark.parametrize("D,G", [(64, 4), (128, 1), (128, 4), (128, 8), (256, 2)])
+@pytest.mark.parametrize("spread", [1e-4, 3e-4, 1e-3, 1e-2])
+def test_decode_of_nearly_equal_scores(rt, S, n, D, G, spread):
+    """Attention that is next to a mean: the result is a small rest of values that cancel.
+
+    Rounding p_t to 11 bits moves a term p_t v_t by at most U_F16 of it, one way or the other as the score's last bits have
+    it.  n such moves add up to U_F16 sqrt(sum (p_t v_t)^2) (their root mean square), which is U_F16 of the result where the
+    values are N(0, 1) and the p_t alike; twice that here.  The result's rounding to bf16 is U_BF16 at most."""
+    cache, q = plain.fill(rt, 1, 2, S, D, 11), _randn(1, 2 * G, D, seed=12)
+    k = plain.values(cache.k_codes[0, :, :n], cache.k_scales[0, :, :n])
+    v = plain.values(cache.v_codes[0, :, :n], cache.v_scales[0, :, :n])
+    s = torch.einsum("hgd,htd->hgt", q[0].double().view(2, G, D), k)
+    scale = spread * math.log(2) / s.std(-1).mean().item()
+    want = torch.einsum("hgt,htd->hgd", torch.softmax(s * scale, -1), v).reshape(2 * G, D)
+    out, lse = rt.kv4_decode(q, cache, kv_len=n, scale=scale)
+    off = (out[0].double() - want).norm(dim=-1) / want.norm(dim=-1)
+    assert off.max() <= plain.U_BF16 + 2 * plain.U_F16, off.max().item()
+    assert (lse[0].double() - torch.logsumexp(s * scale, -1).reshape(-1)).abs().max() <= 32 * plain.U_F32 * (1 + math.log(n))
