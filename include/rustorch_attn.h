@@ -542,7 +542,9 @@ size_t rt_kv4_decode_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_k
  *   q, out : bf16 [B,Hq,D];  lse : NULL or f32 [B,Hq];  kv_lens : device int32 [B] (clamped to max_seq), or NULL
  *   for kv_len_uniform;  scale <= 0 selects 1/sqrt(D).  Hq/Hkv from 1 to 8.  A sequence of length 0 gives
  *   out = 0, lse = -inf.  Queries up to 2^100 in magnitude; a NaN or an infinity in a query makes its row NaN.
- *   lse is as exact as f32 sums are; out is rounded to bf16 from sums of probabilities with 11 bits.  How a sequence
+ *   lse is as exact as f32 sums are; out is rounded to bf16 from sums of probabilities with 11 bits.  A token whose scale
+ *   of a group of V is below 2^-13 of the largest that the group has in the sequence loses bits of that scale (2^-25 of
+ *   the largest at most).  How a sequence
  *   is cut depends on the other sequences' lengths, so that the last bit of a result does too.
  *   weights : NULL or f32 [B,Hkv,max_seq]; weights[b,h,t] += the sum over the query heads of KV head h of the
  *   softmax weight of token t < kv_len (what rt_kv_evict chooses by).

@@ -224,8 +224,18 @@ struct Sums {
     float o[D / 32][2][4];       // [group][0-1, 2-3 of a lane's four dims]: sum p scale c 2^(k - 24), {q 2j, 2j+1} x {c0, c0 + 16 c1}
     float lo[4], lo2[4];         // sum p * lo: row 2i + 1 = group i; see `step` for which of the rows count
     float ref[2], top[2], l[2];  // p = 2^(score - ref); running maximum; sum of p (this lane's tokens)
-    int k;                       // scales are held times 2^k: the largest so far lies in [1/2, 1) (the format's are below 2^14), k <= 15
-    uint32_t scale_limit;        // the largest f16 pattern for which k stands
+    // Of the lanes g = 2i, group i of each span: its scales are held times 2^k, which has the largest so far in [1/2, 1) (the
+    // format's are below 2^14), k <= 15, and scale_limit is the largest f16 pattern for which k stands.  Other lanes' limit is
+    // never passed.
+    int k[D / Kv4Row<D>::kSpan];
+    uint32_t scale_limit[D / Kv4Row<D>::kSpan];
+
+    __device__ __forceinline__ void start(int lane) {
+        *this = {};
+        top[0] = top[1] = -INFINITY;
+#pragma unroll
+        for (uint32_t& limit : scale_limit) limit = lane / 4 % 2 || lane / 8 >= Kv4Row<D>::kSpanGroups ? 0xffffu : 0u;
+    }
 };
 constexpr float kBase = 15.f - kLazy;  // log2 of what p is held times: the largest reaches 2^15
 
@@ -299,15 +309,25 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
                         if (tb * 16 + 8 * r + g < valid) row[tb * 16 + 8 * r + g] = x[tb][2 * r + c] * q.factor[c];
             }
     }
-    uint32_t big = 0;  // the largest scale of V: each lane looks at a token
+    // V and its scales come transposed: 16-bit unit g of a row (4 codes of a group, or a scale or minimum) to the lanes g, those
+    // of tokens 2j and 2j + 1 in one register.
+    // The scales of D = 256 are four matrices for 16 tokens, spans as rows 0-7 and 8-15 of one operand.  Else they are one
+    // for 8 tokens: those of 32 tokens make an operand whose rows 0-7 count in the product with the tokens 0-7 and 16-23,
+    // and rows 8-15 in that with the others.
+    const uint32_t s_at = (uint32_t)__cvta_generic_to_shared(vs) +
+                          (S::kSpans == 2 ? ((lane & 7) + (lane >> 4) * 8) * S::kVScalePitch + (lane >> 3 & 1) * 16 : lane * S::kVScalePitch);
+    uint32_t vw[S::kSpans][4];
 #pragma unroll
-    for (int i = 0; i < S::kGroups; i += S::kSpanGroups) {
-        uint32_t w[S::kSpanGroups];
-        load_words(w, vs + lane * S::kVScalePitch + 4 * i);
+    for (int m = 0; m < S::kSpans; ++m) load_transposed(vw[m], s_at + m * 16 * S::kVScalePitch);
+    uint32_t big[S::kSpans];  // the largest scale of V of this lane's group and tokens, of each span
+    bool larger = false;
 #pragma unroll
-        for (int k = 0; k < S::kSpanGroups; ++k) big = max_half2(big, w[k]);  // and the largest minimum, which is not looked at
+    for (int s = 0; s < S::kSpans; ++s) {
+        const uint32_t m = S::kSpans == 2 ? max_half2(max_half2(vw[0][s], vw[0][2 + s]), max_half2(vw[S::kSpans - 1][s], vw[S::kSpans - 1][2 + s]))
+                                          : max_half2(max_half2(vw[0][0], vw[0][1]), max_half2(vw[0][2], vw[0][3]));
+        big[s] = max(m & 0xffffu, m >> 16);
+        larger |= big[s] > a.scale_limit[s];
     }
-    big &= 0xffffu;
     float top[2];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -316,14 +336,19 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
         m = fmaxf(m, __shfl_xor_sync(kFullMask, m, 8));
         top[c] = fmaxf(m, __shfl_xor_sync(kFullMask, m, 16)) * q.factor[c];
     }
-    if (__any_sync(kFullMask, top[0] > a.top[0] + kLazy || top[1] > a.top[1] + kLazy || big > a.scale_limit)) {
-        big = __reduce_max_sync(kFullMask, big);
-        float grow = 1.f;  // of the scales
-        if (big > a.scale_limit) {
-            const int e = (int)(__float_as_uint(low_half(big)) >> 23) - 127, k = max(-14, min(-1 - e, 15));
-            grow = exp2f((float)(k - a.k));
-            a.k = k;
-            a.scale_limit = (uint32_t)__half_as_ushort(__float2half_rn(exp2f((float)(e + 1)))) - 1;
+    if (__any_sync(kFullMask, top[0] > a.top[0] + kLazy || top[1] > a.top[1] + kLazy || larger)) {
+        float grow[S::kSpans];  // of the scales of this lane's group
+#pragma unroll
+        for (int s = 0; s < S::kSpans; ++s) {
+            uint32_t most = max(big[s], __shfl_xor_sync(kFullMask, big[s], 1));
+            most = max(most, __shfl_xor_sync(kFullMask, most, 2));
+            grow[s] = 1.f;
+            if (most > a.scale_limit[s]) {
+                const int e = (int)(__float_as_uint(low_half(most)) >> 23) - 127, k = max(-14, min(-1 - e, 15));
+                grow[s] = exp2f((float)(k - a.k[s]));
+                a.k[s] = k;
+                a.scale_limit[s] = (uint32_t)__half_as_ushort(__float2half_rn(exp2f((float)(e + 1)))) - 1;
+            }
         }
         float alpha[2];
 #pragma unroll
@@ -337,13 +362,14 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) a.lo[k] *= alpha[k & 1], a.lo2[k] *= alpha[k & 1];
-        alpha[0] *= grow, alpha[1] *= grow;
 #pragma unroll
-        for (int i = 0; i < S::kGroups; ++i)
+        for (int i = 0; i < S::kGroups; ++i) {
+            const float more = __shfl_sync(kFullMask, grow[i / S::kSpanGroups], 8 * (i % S::kSpanGroups));
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) a.o[i][t][k] *= alpha[k & 1];
+                for (int k = 0; k < 4; ++k) a.o[i][t][k] *= alpha[k & 1] * more;
+        }
     }
     uint32_t prob[2][2];  // query g, tokens 2j, 2j + 1 (and 8 more) of a block of 16
 #pragma unroll
@@ -358,29 +384,21 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
         prob[tb][0] = transposed(pack_half2(e[0], e[1]));
         prob[tb][1] = transposed(pack_half2(e[2], e[3]));
     }
-    const uint32_t up = power_half2(a.k);
     const uint32_t rest = kTwice && g < 4 ? 0u : 0xffffffffu;  // 0: this lane's column takes the first parts
-    // V and its scales come transposed: 16-bit unit g of a row (4 codes of a group, or a scale or minimum) to the lanes g, those
-    // of tokens 2j and 2j + 1 in one register.
     const uint32_t v_at = (uint32_t)__cvta_generic_to_shared(vc) + (lane & 15) * S::kVPitch + (lane >> 4) * 16;
-    // The scales of D = 256 are four matrices for 16 tokens, spans as rows 0-7 and 8-15 of one operand.  Else they are one
-    // for 8 tokens: those of 32 tokens make an operand whose rows 0-7 count in the product with the tokens 0-7 and 16-23,
-    // and rows 8-15 in that with the others.
-    const uint32_t s_at = (uint32_t)__cvta_generic_to_shared(vs) +
-                          (S::kSpans == 2 ? ((lane & 7) + (lane >> 4) * 8) * S::kVScalePitch + (lane >> 3 & 1) * 16 : lane * S::kVScalePitch);
     uint32_t f[2][2][S::kSpans];  // [16 tokens][8 tokens][span]
     if constexpr (S::kSpans == 2) {
+        const uint32_t up[2] = {power_half2(a.k[0]), power_half2(a.k[1])};
 #pragma unroll
         for (int tb = 0; tb < 2; ++tb) {
-            uint32_t w[4];
-            load_transposed(w, s_at + tb * 16 * S::kVScalePitch);
+            const uint32_t(&w)[4] = vw[tb];
             mma_f16(a.lo, w[0], w[1], w[2], w[3], prob[tb][0], prob[tb][1]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) f[tb][k / 2][k % 2] = mul_half2(w[k], up);
+            for (int k = 0; k < 4; ++k) f[tb][k / 2][k % 2] = mul_half2(w[k], up[k % 2]);
         }
     } else {
-        uint32_t w[4];
-        load_transposed(w, s_at);
+        const uint32_t up = power_half2(a.k[0]);
+        const uint32_t(&w)[4] = vw[0];
         mma_f16(a.lo, w[0], w[1], w[2], w[3], prob[0][0], prob[1][0]);
         mma_f16(a.lo2, w[0], w[1], w[2], w[3], prob[0][1], prob[1][1]);
 #pragma unroll
@@ -465,9 +483,10 @@ __device__ __forceinline__ void results(const Sums<D>& a, int lane, Row&& row, T
         float l = a.l[c];
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l += __shfl_xor_sync(kFullMask, l, off);
-        const float even = exp2f((float)(24 - a.k)), odd = even * 0.0625f;
 #pragma unroll
         for (int i = 0; i < S::kGroups; ++i) {
+            const int k = __shfl_sync(kFullMask, a.k[i / S::kSpanGroups], 8 * (i % S::kSpanGroups));
+            const float even = exp2f((float)(24 - k)), odd = even * 0.0625f;
             // the minima's sum of the group is with the lanes 2i + 1
             const float sum = S::kSpans == 2 ? a.lo[c + 2 * (i / S::kSpanGroups)] : a.lo[c];
             float y = __shfl_sync(kFullMask, sum, 8 * (i % S::kSpanGroups) + 4 + j);
@@ -548,8 +567,8 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
         for (int i = 0; i < kStages - 1; ++i) prefetch(i, i);
         Queries<D> q;
         q.template load<kTwice>(p, bh, lane);
-        Sums<D> a = {};
-        a.top[0] = a.top[1] = -INFINITY;
+        Sums<D> a;
+        a.start(lane);
         int slot = 0;
         for (int t0 = lo, s = 0; t0 < hi; t0 += kStep, ++s) {
             asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
@@ -638,8 +657,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_cluster_kernel(const DecodePa
         else asm volatile("cp.async.commit_group;" ::: "memory");
     Queries<D> q;
     q.template load<kTwice>(p, bh, lane);
-    Sums<D> a = {};
-    a.top[0] = a.top[1] = -INFINITY;
+    Sums<D> a;
+    a.start(lane);
     int slot = 0, turn = 0;
     const int local = score_steps * kWarps * kStep;  // tokens of a query's scores
     for (int s = first; s < steps; s += every, ++turn) {

@@ -50,3 +50,20 @@ def test_decode_of_nearly_equal_scores(rt, S, n, D, G, spread):
     off = (out[0].double() - want).norm(dim=-1) / want.norm(dim=-1)
     assert off.max() <= plain.U_BF16 + 2 * plain.U_F16, off.max().item()
     assert (lse[0].double() - torch.logsumexp(s * scale, -1).reshape(-1)).abs().max() <= 32 * plain.U_F32 * (1 + math.log(n))
+
+
+@pytest.mark.parametrize("S", [700, 20000])
+@pytest.mark.parametrize("D,G", [(64, 4), (128, 2), (128, 8), (256, 4), (256, 5)])
+def test_decode_of_value_groups_far_apart(rt, S, D, G):
+    """Values of one group 2^18 times those of the next: each group keeps f16's 11 bits of its probabilities and is then
+    rounded to bf16, as `test_decode_of_nearly_equal_scores` has it."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    k, v = (torch.randn(1, 2, S, D, device="cuda", generator=g) for _ in "kv")
+    of = plain.groups(D).cuda()
+    v = v * torch.where(of % 2 == 0, 2.0 ** 11, 2.0 ** -7)
+    cache, q = rt.Kv4Cache(*plain.quantise(k.bfloat16()), *plain.quantise(v.bfloat16())), _randn(1, 2 * G, D, seed=22)
+    out, _ = rt.kv4_decode(q, cache, kv_len=S)
+    want = plain.decode(q, cache, (S,))[0]
+    for i in range(D // 32):
+        off = (out.double() - want)[..., of == i].norm(dim=-1) / want[..., of == i].norm(dim=-1)
+        assert off.max() <= plain.U_BF16 + 2 * plain.U_F16, (i, off.max().item())
