@@ -39,8 +39,10 @@ struct WeighShape {
     static constexpr int kPitch = 2 * D + 64;        // of a query row in shared memory: two rows fill all banks
 };
 
-__device__ __forceinline__ float lse_log2(float lse) {  // a row that saw nothing adds nothing
-    return lse == -INFINITY ? INFINITY : lse * kLog2e;
+__device__ __forceinline__ float lse_log2(float lse) { return lse == -INFINITY ? INFINITY : lse * kLog2e; }
+// A row that saw nothing adds nothing, whatever its query holds.
+__device__ __forceinline__ float weight(float score, float scale_log2, float lse2) {
+    return lse2 == INFINITY ? 0.f : fast_exp2(fmaf(score, scale_log2, -lse2));
 }
 
 // Scores of 16 tokens and 8 query rows, as accumulators of (row t = g or g + 8, queries 2j and 2j + 1).
@@ -94,7 +96,7 @@ __global__ void __launch_bounds__(kThreads) kv_weigh_kernel(const WeighParams p)
             float c[4];
             scores<D>(c, k[m], q);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[m][i / 2] += fast_exp2(fmaf(c[i], p.scale_log2, -l[i & 1]));
+            for (int i = 0; i < 4; ++i) w[m][i / 2] += weight(c[i], p.scale_log2, l[i & 1]);
         }
     } else {
         extern __shared__ __align__(16) uint8_t smem[];
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(kThreads) kv_weigh_kernel(const WeighParams p)
                     scores<D>(c, k[m], q);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        float e = fast_exp2(fmaf(c[i], p.scale_log2, i & 1 ? -l.y : -l.x));
+                        float e = weight(c[i], p.scale_log2, i & 1 ? l.y : l.x);
                         if (!all_seen && t0 + 16 * m + 4 * (i & 2) + g > s_last[n0 + 2 * j + (i & 1)]) e = 0.f;
                         w[m][i / 2] += e;
                     }

@@ -12,6 +12,8 @@
 // What bounds it: no pipe is full.  The exponentials come nearest, 16 a clock and SM (512 clocks a block): that pipe is busy
 // for 40 % of the active clocks, and stalls are fixed latency, TMEM reads, shared memory and barriers, in this order.  They are
 // ex2's, not a short polynomial's, since the weights are f32 sums.
+#include <climits>
+
 #include "cache_kernels.h"
 #include "kernels.h"
 #include "tc_ptx.cuh"
@@ -46,6 +48,17 @@ struct WeighTc {
     static constexpr int kKeys = kTile * D * 2, kKeySub = kTile * 128, kQueries = kRows * D * 2, kQuerySub = kRows * 128, kSubs = D / 64;
     static constexpr int kSmem = kKeys + kRing * kQueries + 1024;  // and their alignment
 };
+
+// Barrier of the epilogue's warps, and whether `x` holds in any of their threads.
+__device__ __forceinline__ bool barrier_or(bool x) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, 1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)x), "n"(kEpilogue)
+        : "memory");
+    return any;
+}
 
 // A token's scores of a block of rows: their exponentials into `sum`.  The buffer is handed back once it is in registers.
 template <bool kHidden>
@@ -198,15 +211,15 @@ __global__ void __launch_bounds__(kThreads) kv_weigh_tc_kernel(const __grid_cons
             float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
             for (int block = 0; block < blocks; ++block, ++u) {
                 const int slot = u % kRing, rows_slot = u & 1;
-                const bool hidden = !all_seen || (int64_t)(block + 1) * kRows > rows;
+                bool hidden = !all_seen;
                 if (tid < kRows) {  // what the block before last read from these places is two barriers ago
-                    s_lse[rows_slot][tid] = next == -INFINITY ? -INFINITY : -next * kLog2e;
-                    if (hidden) {
-                        const unsigned r = (unsigned)block * kRows + tid;
-                        s_last[rows_slot][tid] = r < rows ? (int)(len - p.seq_q + r % (unsigned)p.seq_q) : -1;
-                    }
+                    const bool none = next == -INFINITY;  // its query may be anything, so that the test and not the exponent hides it
+                    s_lse[rows_slot][tid] = none ? 0.f : -next * kLog2e;
+                    const unsigned r = (unsigned)block * kRows + tid;
+                    s_last[rows_slot][tid] = none ? -1 : all_seen ? INT_MAX : (int)(len - p.seq_q + r % (unsigned)p.seq_q);
+                    hidden |= none;
                 }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                hidden = barrier_or(hidden);
                 next = row_lse(block + 1 < blocks ? block + 1 : 0);
                 if (ok) ok = __all_sync(kFullMask, mbar_wait(&scores_full[slot], (u / kRing) & 1, p.status, kToScores));
                 if (!ok) continue;  // the other warps' barriers still count on this one

@@ -67,3 +67,28 @@ def test_decode_of_value_groups_far_apart(rt, S, D, G):
     for i in range(D // 32):
         off = (out.double() - want)[..., of == i].norm(dim=-1) / want[..., of == i].norm(dim=-1)
         assert off.max() <= plain.U_BF16 + 2 * plain.U_F16, (i, off.max().item())
+
+
+# ------------------------------------------------------------------------------------------------ weights
+
+
+@pytest.mark.parametrize("T,D", [(1, 64), (1, 128), (1, 256), (5, 64), (5, 128), (7, 256), (40, 64), (40, 128), (64, 256), (150, 128)])
+@pytest.mark.parametrize("junk", [math.nan, math.inf])
+def test_weigh_of_rows_that_saw_nothing(rt, T, D, junk):
+    """A row whose lse is -inf adds nothing, whatever its query holds: the rows of a batch's padding."""
+    B, Hq, Hkv, S = 2, 8, 2, 400
+    lens = (400, 211)
+    q, k = _randn(B, Hq, T, D, seed=1), _randn(B, Hkv, S, D, seed=2)
+    s = torch.einsum("bhqd,bhtd->bhqt", q.double(), k.double().repeat_interleave(Hq // Hkv, 1)) / math.sqrt(D)
+    lse = torch.logsumexp(s, -1).float()
+    gone = torch.rand(B, Hq, T, device="cuda", generator=torch.Generator(device="cuda").manual_seed(3)) < 0.4
+    gone[:, 0], gone[:, 1] = True, False  # in every group some and not all
+    lse[gone] = -math.inf
+    w = torch.zeros(B, Hkv, S, device="cuda")
+    want, tol = plain.weigh(q, k, lse, lens)
+    bad = torch.where(gone[..., None], torch.full_like(q, junk), q)
+    if T == 1:
+        rt.kv_weigh(bad[:, :, 0].contiguous(), k, lse[:, :, 0].contiguous(), w, kv_lens=_i32(*lens))
+    else:
+        rt.kv_weigh(bad, k, lse, w, kv_lens=_i32(*lens))
+    assert ((w.double() - want).abs() <= tol + 2 * plain.U_F32 * (1 + want)).all()
