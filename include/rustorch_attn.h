@@ -578,7 +578,8 @@ int rt_kv_weigh_bf16(const void* q, const void* k_cache, const float* lse, float
  * they were.
  *   n_planes (1 to 4) pairs of planes src[i] [B,Hkv,max_seq,row_bytes[i]] -> dst[i] [B,Hkv,max_seq_out,row_bytes[i]]:
  *       K and V of a bf16 cache, or the four planes of a 4-bit one; HOST arrays; row_bytes multiples of 8, up to
- *       4096; planes 16-byte aligned and none of src overlapping one of dst (nor weights weights_out, nor kv_lens lens_out).
+ *       4096; planes 16-byte aligned.  Nothing that is written (dst, weights_out, kept, lens_out) may overlap what is
+ *       read (src, weights, kv_lens) or anything else that is written.
  *   weights : f32 [B,Hkv,max_seq];  weights_out : f32 [B,Hkv,max_seq_out], the kept rows' weights, zero behind them.
  *   kept    : int32 [B,Hkv,keep], the rows' places in the source, -1 behind them;
  *   lens_out : int32 [B], min(kv_len, keep).

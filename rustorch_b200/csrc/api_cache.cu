@@ -31,9 +31,13 @@ inline int check_shape(int64_t batch, int64_t n_kv, int head_dim, int64_t max_se
     return RT_OK;
 }
 
-inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
-    const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + b_bytes && y < x + a_bytes;
+struct Bytes {
+    const void* at;
+    size_t n;
+};
+inline bool overlap(const Bytes& a, const Bytes& b) {
+    const auto x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+    return x < y + b.n && y < x + a.n;
 }
 
 }  // namespace
@@ -158,12 +162,25 @@ int rt_kv_evict(const void* const* src, void* const* dst, const int32_t* row_byt
         if (!aligned16(src[i]) || !aligned16(dst[i])) return RT_ERR_ALIGNMENT;
         p.src[i] = src[i], p.dst[i] = dst[i], p.row_bytes[i] = row_bytes[i];
     }
-    // the move has no order: a row that is written must be none that is still read
-    for (int i = 0; i < n_planes; ++i)
-        for (int j = 0; j < n_planes; ++j)
-            if (overlap(src[i], rows_in * row_bytes[i], dst[j], rows_out * row_bytes[j])) return RT_ERR_UNSUPPORTED;
-    if (overlap(weights, rows_in * sizeof(float), weights_out, rows_out * sizeof(float))) return RT_ERR_UNSUPPORTED;
-    if (kv_lens && overlap(kv_lens, batch * sizeof(int32_t), lens_out, batch * sizeof(int32_t))) return RT_ERR_UNSUPPORTED;
+    // The selection and the move have no order: what is written must be nothing that is read, and nothing twice.
+    constexpr int kMost = rt::EvictPlanes::kMost;
+    Bytes read[kMost + 2], written[kMost + 3];
+    int n_read = 0, n_written = 0;
+    for (int i = 0; i < n_planes; ++i) {
+        read[n_read++] = {src[i], rows_in * row_bytes[i]};
+        written[n_written++] = {dst[i], rows_out * row_bytes[i]};
+    }
+    read[n_read++] = {weights, rows_in * sizeof(float)};
+    if (kv_lens) read[n_read++] = {kv_lens, batch * sizeof(int32_t)};
+    written[n_written++] = {weights_out, rows_out * sizeof(float)};
+    written[n_written++] = {kept, (size_t)(batch * n_kv_heads) * keep * sizeof(int32_t)};
+    written[n_written++] = {lens_out, batch * sizeof(int32_t)};
+    for (int i = 0; i < n_written; ++i) {
+        for (int j = 0; j < n_read; ++j)
+            if (overlap(written[i], read[j])) return RT_ERR_UNSUPPORTED;
+        for (int j = 0; j < i; ++j)
+            if (overlap(written[i], written[j])) return RT_ERR_UNSUPPORTED;
+    }
     return (int)rt::launch_kv_evict(p, weights, weights_out, kept, lens_out, batch, (int)n_kv_heads, max_seq, max_seq_out,
                                     kv_lens, kv_len_uniform, keep, recent, as_stream(stream));
 }

@@ -57,7 +57,7 @@ def kv_evict(cache, out, weights, keep: int, recent: int = 0, kv_lens=None, kv_l
     (``rt_kv_evict``).
 
     ``cache`` and ``out``: two ``Kv4Cache``, or two pairs (k_cache, v_cache) of bf16 ``[B,Hkv,max_seq,D]`` tensors; ``out`` holds
-    at least ``keep`` rows, shares no memory with ``cache``, and has its other rows left as they were.  ``weights`` f32
+    at least ``keep`` rows, shares no memory with ``cache`` nor one of its tensors with another, and has its other rows left as they were.  ``weights`` f32
     ``[B,Hkv,max_seq]``.  Returns (lens int32 ``[B]``, the lengths in ``out``; weights_out f32 ``[B,Hkv,max_seq of out]``, the
     rows' weights, zero behind them; kept int32 ``[B,Hkv,keep]``, the rows' places in ``cache``, -1 behind them)."""
     if type(cache) is type(out) and type(cache) in (Kv4Cache, tuple):
