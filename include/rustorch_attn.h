@@ -541,7 +541,8 @@ size_t rt_kv4_decode_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_k
  * Batched single-token GQA decode over a 4-bit cache: softmax(scale * q K^T) V of the values the codes stand for.
  *   q, out : bf16 [B,Hq,D];  lse : NULL or f32 [B,Hq];  kv_lens : device int32 [B] (clamped to max_seq), or NULL
  *   for kv_len_uniform;  scale <= 0 selects 1/sqrt(D).  Hq/Hkv from 1 to 8.  A sequence of length 0 gives
- *   out = 0, lse = -inf.  Queries up to 2^100 in magnitude; a NaN or an infinity in a query makes its row NaN.
+ *   out = 0, lse = -inf.  Queries up to 2^100 in magnitude; a NaN or an infinity in a query makes its row NaN; a value
+ *   below 2^-27 of its query's largest is off by up to 2^-35 of the largest.
  *   lse is as exact as f32 sums are; out is rounded to bf16 from sums of probabilities with 11 bits.  A token whose scale
  *   of a group of V is below 2^-13 of the largest that the group has in the sequence loses bits of that scale (2^-25 of
  *   the largest at most).  How a sequence

@@ -151,8 +151,9 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[kWords], const uint8_t*
 }
 
 // One (sequence, KV head)'s queries as the B operand of the score products: lane (g, j) = (lane / 4, lane % 4) holds query
-// g's octets of quarter j; with kTwice, queries 0 to 3 again as 4 to 7.  The queries are scaled by a power of two that brings their largest value to 2^14, where
-// bf16's 8 bits fit f16 exactly (values 2^-31 of the largest and smaller lose bits).
+// g's octets of quarter j; with kTwice, queries 0 to 3 again as 4 to 7.  The queries are scaled by a power of two that brings
+// their largest value to 2^14, where bf16's 8 bits fit f16 exactly down to 2^-31 of the largest, and to 2^-27 at the odd
+// places, which are held 16 times smaller.  Smaller values are off by half of f16's last place at most, 2^-35 of the largest there.
 template <int D>
 struct Queries {
     uint32_t even[Shape<D>::kGroups][2], odd[Shape<D>::kGroups][2];  // pairs (0,4), (2,6) and (1,5)/16, (3,7)/16 of an octet

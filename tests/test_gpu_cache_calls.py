@@ -69,6 +69,30 @@ def test_decode_of_value_groups_far_apart(rt, S, D, G):
         assert off.max() <= plain.U_BF16 + 2 * plain.U_F16, (i, off.max().item())
 
 
+@pytest.mark.parametrize("S", [700, 20000])
+@pytest.mark.parametrize("D,G,at", [(64, 4, 3), (128, 1, 0), (128, 8, 77), (256, 4, 200)])
+@pytest.mark.parametrize("far", [20, 26, 28, 31])
+def test_decode_of_queries_with_one_large_value(rt, S, D, G, at, far):
+    """One value 2^far times the others, at a place where all keys are zero: the others make the scores.
+
+    Odd places are held in f16 16 times smaller than even ones, the largest value in [2^14, 2^15): f16's last place, 2^-24, is
+    2^-34 of the largest there, and half of it is lost of a value, which meets codes of up to 15 scales; a group's sum of
+    32 values, in units of 64, loses 2^-33 of the largest, less than the 32 values' 2^-35 each, and meets the minimum."""
+    of = plain.groups(D).cuda()
+    g = torch.Generator(device="cuda").manual_seed(31)
+    k, v = (torch.randn(1, 2, S, D, device="cuda", generator=g) for _ in "kv")
+    k[..., of == of[at]] = 0
+    cache, q = rt.Kv4Cache(*plain.quantise(k.bfloat16()), *plain.quantise(v.bfloat16())), _randn(1, 2 * G, D, seed=32)
+    q[:, :, at] = 2.0 ** far
+    out, lse = rt.kv4_decode(q, cache, kv_len=S)
+    want, want_lse, _, out_tol, lse_tol, _ = plain.decode(q, cache, (S,))
+    scales = cache.k_scales[0].double().abs()
+    lost = (2.0 ** (far - 35) * 32 / math.sqrt(D) * (15 * scales[..., 0] + scales[..., 1]).sum(-1)).amax(-1).repeat_interleave(G)
+    values = (plain.values(cache.v_codes[0], cache.v_scales[0]).abs() + 15 * cache.v_scales[0, ..., 0].double()[..., of]).amax(1).repeat_interleave(G, 0)
+    assert ((lse[0].double() - want_lse[0]).abs() <= lse_tol[0] + lost).all()
+    assert ((out[0].double() - want[0]).abs() <= out_tol[0] + 2 * lost[:, None] * values).all()
+
+
 # ------------------------------------------------------------------------------------------------ weights
 
 
