@@ -7,11 +7,13 @@
 // tokens, 32 heads on 8, D = 128, took 24.3 us with rings of two and 24.1 with these; the mask's test compiled apart from
 // the blocks without one brought 21.7).  A token is a TMEM lane, so a thread of the four epilogue warps has a token's scores
 // to itself: it adds up their exponentials in a register, with the rows' log-sum-exps broadcast from shared memory,
-// and writes the token's weight once.  One thread issues all loads and products.  Two CTAs an SM.
+// and writes the token's weight once.  One thread issues all loads and products.  Two CTAs an SM, at D = 256
+// one.
 //
 // What bounds it: no pipe is full.  The exponentials come nearest, 16 a clock and SM (512 clocks a block): that pipe is busy
 // for 40 % of the active clocks, and stalls are fixed latency, TMEM reads, shared memory and barriers, in this order.  They are
 // ex2's, not a short polynomial's, since the weights are f32 sums.
+#include <algorithm>
 #include <climits>
 
 #include "cache_kernels.h"
@@ -47,6 +49,7 @@ struct WeighTc {
     // 64 columns are a swizzled piece
     static constexpr int kKeys = kTile * D * 2, kKeySub = kTile * 128, kQueries = kRows * D * 2, kQuerySub = kRows * 128, kSubs = D / 64;
     static constexpr int kSmem = kKeys + kRing * kQueries + 1024;  // and their alignment
+    static constexpr int kPerSm = 2 * kSmem <= 224 * 1024 ? 2 : 1;  // CTAs that an SM's shared memory holds
 };
 
 // Barrier of the epilogue's warps, and whether `x` holds in any of their threads.
@@ -256,11 +259,13 @@ cudaError_t launch_kv_weigh_tc(const void* q, const void* k_cache, const float* 
     p.lse = lse, p.weights = weights, p.max_seq = max_seq, p.seq_q = seq_q, p.kv_lens = kv_lens, p.kv_len = (int)kv_len_uniform;
     p.n_kv = n_kv, p.group = n_heads / n_kv, p.scale_log2 = scale * kLog2e, p.status = device_status_ptr();
     if (!p.status) return cudaErrorInvalidSymbol;
-    // two CTAs an SM in all, or one for every tile
-    const int64_t tiles = (longest + kTile - 1) / kTile, each = (2 * sm_count() + groups - 1) / groups;
-    const dim3 grid((unsigned)(tiles < each ? tiles : each), n_kv, (unsigned)batch);
     return for_head_dim(head_dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
+        // No more CTAs than are resident at a time (one for every tile, or one a head, where these are fewer or more): a second
+        // wave of a few waits for all of the first.  The other side is two an SM at every D, rounded up: at D = 256, 256 rows,
+        // 8 heads of 16,001 tokens 29.3 and 34.2 us, 12 of 20,000 61.1 and 75.9; D = 128, 56 heads of 8000 62.4 and 83.6.
+        const int64_t tiles = (longest + kTile - 1) / kTile, each = std::max<int64_t>(1, WeighTc<D>::kPerSm * sm_count() / groups);
+        const dim3 grid((unsigned)(tiles < each ? tiles : each), n_kv, (unsigned)batch);
         const cudaError_t e = set_max_dynamic_smem_once<kv_weigh_tc_kernel<D>>(WeighTc<D>::kSmem);
         if (e != cudaSuccess) return e;
         return launch_chained(kv_weigh_tc_kernel<D>, grid, kThreads, (size_t)WeighTc<D>::kSmem, stream, map_k, map_q, p);
