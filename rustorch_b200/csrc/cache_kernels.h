@@ -60,7 +60,7 @@ cudaError_t launch_kv_weigh(const void* q, const void* k_cache, const float* lse
                             int n_kv, int64_t seq_q, int head_dim, int64_t max_seq, const int32_t* kv_lens,
                             int64_t kv_len_uniform, float scale, cudaStream_t stream);
 
-// ---- kv_weigh_tc.cu: the same on tcgen05; cudaErrorNotSupported = not covered
+// ---- kv_weigh_tc.cu: the same on tcgen05, for the rows from which it is faster
 cudaError_t launch_kv_weigh_tc(const void* q, const void* k_cache, const float* lse, float* weights, int64_t batch, int n_heads,
                                int n_kv, int64_t seq_q, int head_dim, int64_t max_seq, int64_t longest, const int32_t* kv_lens,
                                int64_t kv_len_uniform, float scale, cudaStream_t stream);

@@ -15,11 +15,10 @@ namespace rt {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kBlock = 64;  // query rows in shared memory at a time
 // Query rows of a KV head from which kv_weigh_tc.cu's kernel is taken.  8 heads of 16,001 tokens, here and there: D = 128, 32
 // rows 10.4 and 9.5 us, 64 rows 13.1 and 8.7, 128 rows 20.6 and 12.8; D = 64, 32 rows 8.1 and 8.5 (16 x 2000 tokens: 11.9 and
 // 16.2), 64 rows 10.6 and 8.1; D = 256, 32 rows 22.9 and 15.8.
-constexpr int tensor_rows(int head_dim) { return head_dim == 64 ? 64 : 32; }
+__host__ __device__ constexpr int tensor_rows(int head_dim) { return head_dim == 64 ? 64 : 32; }
 
 struct WeighParams {
     const __nv_bfloat16 *q, *k;
@@ -99,44 +98,38 @@ __global__ void __launch_bounds__(kThreads) kv_weigh_kernel(const WeighParams p)
             for (int i = 0; i < 4; ++i) w[m][i / 2] += weight(c[i], p.scale_log2, l[i & 1]);
         }
     } else {
+        constexpr int kRows = tensor_rows(D);  // of which there are fewer
         extern __shared__ __align__(16) uint8_t smem[];
-        __shared__ float s_lse[kBlock];
-        __shared__ int s_last[kBlock];  // the last token that a row sees
-        const int64_t rows = p.group * p.seq_q;
+        __shared__ float s_lse[kRows];
+        __shared__ int s_last[kRows];  // the last token that a row sees
+        const int rows = p.group * (int)p.seq_q;
         // the first query's place: whether any row of this warp's tokens can be hidden
         const bool all_seen = t0 + 16 * S::kTiles - 1 <= len - p.seq_q;
-        for (int64_t r0 = 0; r0 < rows; r0 += kBlock) {
-            const int n_rows = (int)min((int64_t)kBlock, rows - r0);
-            __syncthreads();
-            for (int i = tid; i < kBlock * (D / 8); i += kThreads) {
-                const int r = i / (D / 8), c = i % (D / 8);
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (r < n_rows) x = *reinterpret_cast<const uint4*>(p.q + (row0 + r0 + r) * D + 8 * c);
-                *reinterpret_cast<uint4*>(smem + r * S::kPitch + 16 * c) = x;
-            }
-            if (tid < kBlock) {
-                const int64_t r = r0 + tid;
-                s_lse[tid] = tid < n_rows ? lse_log2(p.lse[row0 + r]) : INFINITY;
-                s_last[tid] = (int)(len - p.seq_q + r % p.seq_q);
-            }
-            __syncthreads();
-            if (t0 >= len) continue;
-            for (int n0 = 0; n0 < n_rows; n0 += 8) {
-                uint4 q[S::kChunks];
+        for (int i = tid; i < kRows * (D / 8); i += kThreads) {
+            const int r = i / (D / 8), c = i % (D / 8);
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (r < rows) x = *reinterpret_cast<const uint4*>(p.q + (row0 + r) * D + 8 * c);
+            *reinterpret_cast<uint4*>(smem + r * S::kPitch + 16 * c) = x;
+        }
+        if (tid < kRows) {
+            s_lse[tid] = tid < rows ? lse_log2(p.lse[row0 + tid]) : INFINITY;
+            s_last[tid] = len - (int)p.seq_q + tid % (int)p.seq_q;
+        }
+        __syncthreads();
+        for (int n0 = 0; n0 < rows; n0 += 8) {
+            uint4 q[S::kChunks];
 #pragma unroll
-                for (int n = 0; n < S::kChunks; ++n)
-                    q[n] = *reinterpret_cast<const uint4*>(smem + (n0 + g) * S::kPitch + 64 * n + 16 * j);
-                const float2 l = *reinterpret_cast<const float2*>(&s_lse[n0 + 2 * j]);
+            for (int n = 0; n < S::kChunks; ++n) q[n] = *reinterpret_cast<const uint4*>(smem + (n0 + g) * S::kPitch + 64 * n + 16 * j);
+            const float2 l = *reinterpret_cast<const float2*>(&s_lse[n0 + 2 * j]);
 #pragma unroll
-                for (int m = 0; m < S::kTiles; ++m) {
-                    float c[4];
-                    scores<D>(c, k[m], q);
+            for (int m = 0; m < S::kTiles; ++m) {
+                float c[4];
+                scores<D>(c, k[m], q);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        float e = weight(c[i], p.scale_log2, i & 1 ? l.y : l.x);
-                        if (!all_seen && t0 + 16 * m + 4 * (i & 2) + g > s_last[n0 + 2 * j + (i & 1)]) e = 0.f;
-                        w[m][i / 2] += e;
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    float e = weight(c[i], p.scale_log2, i & 1 ? l.y : l.x);
+                    if (!all_seen && t0 + 16 * m + 4 * (i & 2) + g > s_last[n0 + 2 * j + (i & 1)]) e = 0.f;
+                    w[m][i / 2] += e;
                 }
             }
         }
@@ -164,17 +157,15 @@ cudaError_t launch_kv_weigh(const void* q, const void* k_cache, const float* lse
     p.n_kv = n_kv, p.group = n_heads / n_kv, p.scale_log2 = scale * kLog2e;
     const int64_t longest = kv_lens ? max_seq : kv_len_uniform;
     if (longest == 0) return cudaSuccess;
-    if (p.group * seq_q >= tensor_rows(head_dim) && seq_q > 1) {
-        const cudaError_t e = launch_kv_weigh_tc(q, k_cache, lse, weights, batch, n_heads, n_kv, seq_q, head_dim, max_seq, longest, kv_lens,
-                                                 kv_len_uniform, scale, stream);
-        if (e != cudaErrorNotSupported) return e;
-    }
+    if (p.group * seq_q >= tensor_rows(head_dim))
+        return launch_kv_weigh_tc(q, k_cache, lse, weights, batch, n_heads, n_kv, seq_q, head_dim, max_seq, longest, kv_lens, kv_len_uniform,
+                                  scale, stream);
     return for_head_dim(head_dim, [&](auto d) {
         constexpr int D = decltype(d)::value;
         using S = WeighShape<D>;
         const dim3 grid((unsigned)((longest + S::kTokens - 1) / S::kTokens), n_kv, (unsigned)batch);
         if (seq_q == 1) return launch_chained(kv_weigh_kernel<D, true>, grid, kThreads, 0, stream, p);
-        return launch_chained(kv_weigh_kernel<D, false>, grid, kThreads, (size_t)kBlock * S::kPitch, stream, p);
+        return launch_chained(kv_weigh_kernel<D, false>, grid, kThreads, (size_t)tensor_rows(D) * S::kPitch, stream, p);
     });
 }
 
