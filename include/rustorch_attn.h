@@ -545,8 +545,8 @@ size_t rt_kv4_decode_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_k
  *   below 2^-27 of its query's largest is off by up to 2^-35 of the largest.
  *   lse is as exact as f32 sums are; out is rounded to bf16 from sums of probabilities with 11 bits.  A token whose scale
  *   of a group of V is below 2^-13 of the largest that the group has in the sequence loses bits of that scale (2^-25 of
- *   the largest at most).  How a sequence
- *   is cut depends on the other sequences' lengths, so that the last bit of a result does too.
+ *   the largest at most).  How a sequence is cut depends on the other sequences' lengths and on whether weights are
+ *   asked for, so that the last bit of a result does too.
  *   weights : NULL or f32 [B,Hkv,max_seq]; weights[b,h,t] += the sum over the query heads of KV head h of the
  *   softmax weight of token t < kv_len (what rt_kv_evict chooses by).
  */

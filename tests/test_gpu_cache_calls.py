@@ -4,6 +4,7 @@ import math
 import pytest
 
 from tests import kv4_plain as plain
+from tests.test_gpu_kv4 import _check, _decode_case
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -21,10 +22,6 @@ def _i32(*v):
 
 def _randn(*shape, seed=0, scale=1.0):
     return (torch.randn(shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)) * scale).bfloat16()
-
-
-def _cut(cache, n):
-    return type(cache)(*(t[:, :, :n].contiguous() for t in cache))
 
 
 # ------------------------------------------------------------------------------------------------ decode
@@ -93,6 +90,149 @@ def test_decode_of_queries_with_one_large_value(rt, S, D, G, at, far):
     assert ((out[0].double() - want[0]).abs() <= out_tol[0] + 2 * lost[:, None] * values).all()
 
 
+# Below, what runs in one launch of clusters at the sizes of tests/test_gpu_kv4.py is run where the workers take it: more than 8192
+# rows of cache, or more (sequence, KV head) pairs than half the SMs, and several steps a worker.
+@pytest.mark.parametrize("B,S", [(40, 3000), (1, 60000)])
+@pytest.mark.parametrize("what", ["far scores", "growing scores", "falling scores", "one token", "large q", "small q", "tiny v", "huge v",
+                                  "mixed v", "growing v", "scale"])
+def test_decode_of_wide_ranges_in_runs(rt, what, B, S):
+    Hq, Hkv, D = 8, 2, 128
+    g = torch.Generator(device="cuda").manual_seed(8)
+    k, v = (torch.randn(B, Hkv, S, D, device="cuda", generator=g) for _ in "kv")
+    along = torch.arange(S, device="cuda")[:, None] / S
+    q, scale = _randn(B, Hq, D, seed=9), None
+    if what == "far scores":
+        k = k * 30
+    elif what == "growing scores":
+        k = k * (40 * along)
+    elif what == "falling scores":
+        k = k * (40 - 40 * along)
+    elif what == "one token":
+        k[:, :, 333] += 8 * q.view(B, Hkv, -1, D)[:, :, 0].float()
+    elif what == "large q":
+        q, scale = (q.float() * 2.0 ** 60).bfloat16(), 2.0 ** -62
+    elif what == "small q":
+        q, scale = (q.float() * 2.0 ** -90).bfloat16(), 2.0 ** 88
+    elif what == "tiny v":
+        v = v * 2e-4
+    elif what == "huge v":
+        v = v * 9000
+    elif what == "mixed v":
+        v[:, :, ::3] *= 4000
+    elif what == "growing v":
+        v = v * torch.exp2(18 * along - 6)
+    else:
+        scale = 0.7
+    cache = rt.Kv4Cache(*plain.quantise(k.bfloat16()), *plain.quantise(v.bfloat16()))
+    _decode_case(rt, B, Hq, Hkv, D, S, tuple(S - 31 * b for b in range(B)), scale=scale, q=q, cache=cache)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n", [8191, 8192, 8193])
+@pytest.mark.parametrize("B", [1, 9])
+def test_decode_on_both_sides_of_the_longest_cluster(rt, B, n, D):
+    """Weighed and not, as many rows of cache as tokens, then fewer tokens than the cache has room for.  Weights can change how
+    a sequence is cut, so that each call is held against 64 bits and not against the other."""
+    for Hq, lens in ((8, (n,) * B), (16, tuple(n - 900 * b - 1 for b in range(B)))):
+        cache, q = plain.fill(rt, B, 2, n, D, n), _randn(B, Hq, D, seed=n + 50)
+        o, l, w, ot, lt, wt = plain.decode(q, cache, lens)
+        for weights in (None, torch.zeros(B, 2, n, device="cuda")):
+            kw = dict(kv_len=n) if lens[-1] == n else dict(kv_lens=_i32(*lens))
+            out, lse = rt.kv4_decode(q, cache, weights=weights, **kw)
+            _check(out, o, ot, "out")
+            _check(lse, l, lt, "lse")
+        _check(weights, w, wt + 2 * plain.U_F32 * (1 + w), "weights")
+
+
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 8, 8), (128, 32, 8), (256, 8, 1)])
+def test_decode_of_a_cache_much_larger_than_its_sequences(rt, D, Hq, Hkv):
+    _decode_case(rt, 3, Hq, Hkv, D, 131072, (1000, 33, 257), seed=3)
+
+
+def test_decode_in_runs_does_not_read_rows_behind_the_length(rt):
+    lens = tuple(100 + 37 * b for b in range(45))
+    cache, q = plain.fill(rt, 45, 2, 2000, 128, 5), _randn(45, 8, 128, seed=6)
+    want = rt.kv4_decode(q, cache, kv_lens=_i32(*lens))
+    for b, n in enumerate(lens):
+        cache[1][b, :, n:], cache[3][b, :, n:] = math.nan, math.inf
+    got = rt.kv4_decode(q, cache, kv_lens=_i32(*lens))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("B,S", [(40, 3000), (2, 20001)])
+def test_decode_in_runs_keeps_to_its_workspace(rt, B, S):
+    """Scratch of exactly the size that is asked for, full of ones: the bytes around it stay."""
+    Hq, Hkv, D = 8, 2, 64
+    lens = tuple(S - 61 * b for b in range(B))
+    cache, q = plain.fill(rt, B, Hkv, S, D, 3), _randn(B, Hq, D, seed=4)
+    for weighed in (False, True):
+        weights = torch.zeros(B, Hkv, S, device="cuda") if weighed else None
+        need = rt.kv4_workspace_bytes(B, Hq, Hkv, D, S, weighed)
+        assert need > 0
+        room = torch.full((need + 4096,), 255, dtype=torch.uint8, device="cuda")
+        out, lse = torch.full_like(q, math.nan), torch.full((B, Hq), math.nan, device="cuda")
+        rt.kv4_decode(q, cache, kv_lens=_i32(*lens), weights=weights, workspace=room[2048:2048 + need], out=out, lse=lse)
+        assert (room[:2048] == 255).all() and (room[2048 + need:] == 255).all()
+        o, l, w, ot, lt, wt = plain.decode(q, cache, lens)
+        _check(out, o, ot, "out")
+        _check(lse, l, lt, "lse")
+        if weighed:
+            _check(weights, w, wt + 2 * plain.U_F32 * (1 + w), "weights")
+
+
+@pytest.mark.parametrize("B,S", [(40, 3000), (2, 20001)])
+def test_decode_in_runs_on_streams_and_in_graphs(rt, B, S):
+    """Two streams at once, and two graphs that share a pool, replayed with lengths that change: decode, merge and weights."""
+    Hq, Hkv, D = 8, 2, 128
+    caches = [plain.fill(rt, B, Hkv, S, D, s) for s in (1, 2)]
+    qs = [_randn(B, Hq, D, seed=s) for s in (3, 4)]
+    lens = [_i32(*(S - 7 * b for b in range(B))), _i32(*(5 + 13 * b for b in range(B)))]
+
+    def call(i, **kw):
+        w = torch.zeros(B, Hkv, S, device="cuda")
+        return *rt.kv4_decode(qs[i], caches[i], kv_lens=lens[i], weights=w, **kw), w
+    want = [call(i) for i in (0, 1)]
+    for i in (0, 1):
+        o, l, w, ot, lt, wt = plain.decode(qs[i], caches[i], lens[i].tolist())
+        for got, ref, tol, what in zip(want[i], (o, l, w), (ot, lt, wt + 2 * plain.U_F32 * (1 + w)), ("out", "lse", "weights")):
+            _check(got, ref, tol, what)
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in "ab"], [None, None]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = call(i)
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        assert all(torch.equal(a, b) for a, b in zip(got[i], want[i]))
+    pool, graphs, outs = torch.cuda.graph_pool_handle(), [], []
+    for i in (0, 1):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(call(i))
+        graphs.append(graph)
+    for swap in (False, True):
+        if swap:
+            a = lens[0].clone()
+            lens[0].copy_(lens[1])
+            lens[1].copy_(a)
+        for i in (0, 1):
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], call(i)))
+
+
+def test_read_into_tensors_of_the_caller(rt):
+    cache = plain.fill(rt, 2, 3, 50, 128, 9)
+    want = rt.kv4_read(cache, 20, start=7, kv_lens=_i32(50, 12))
+    out = tuple(torch.full((2, 3, 20, 128), math.nan, dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    got = rt.kv4_read(cache, 20, start=7, kv_lens=_i32(50, 12), out=out)
+    assert got[0] is out[0] and got[1] is out[1]
+    for g, w, i in zip(got, want, (0, 2)):
+        rows = plain.values(cache[i], cache[i + 1], torch.float32).bfloat16()[:, :, 7:27]
+        assert torch.equal(g, w) and torch.equal(g[0], rows[0]) and torch.equal(g[1, :, :5], rows[1, :, :5]) and not g[1, :, 5:].any()
+
+
 # ------------------------------------------------------------------------------------------------ weights
 
 
@@ -116,3 +256,60 @@ def test_weigh_of_rows_that_saw_nothing(rt, T, D, junk):
     else:
         rt.kv_weigh(bad, k, lse, w, kv_lens=_i32(*lens))
     assert ((w.double() - want).abs() <= tol + 2 * plain.U_F32 * (1 + want)).all()
+
+
+# 296 CTAs at most (148 at D = 256) share the tiles of 128 tokens: here the longest sequences have 4 to 10 for each.  1, 4, 5 and
+# 17 blocks of 64 query rows; sequences shorter than their queries, and tiles in which the last queries hide tokens.
+@pytest.mark.parametrize("B,Hq,Hkv,T,D,S,lens", [
+    (8, 64, 8, 8, 128, 3000, (3000, 1, 127, 128, 129, 2000, 385, 2999)),
+    (8, 32, 8, 64, 64, 3000, (3000, 1500, 63, 2900, 129, 2000, 2561, 2999)),
+    (8, 32, 8, 80, 128, 3000, (79, 2560, 3000, 2900, 2561, 2000, 2816, 2999)),
+    (4, 16, 8, 160, 256, 5000, (5000, 159, 4001, 2048)),
+    (2, 8, 1, 136, 256, 40000, (40000, 33333)),
+    (1, 16, 2, 136, 64, 100000, (99999,)),
+])
+def test_weigh_of_many_tiles_a_cta(rt, B, Hq, Hkv, T, D, S, lens):
+    q, k = _randn(B, Hq, T, D, seed=1), _randn(B, Hkv, S, D, seed=2)
+    lse = torch.full((B, Hq, T), 7.5, device="cuda") + torch.rand(B, Hq, T, device="cuda")
+    before = torch.rand(B, Hkv, S, device="cuda")
+    w = before.clone()
+    rt.kv_weigh(q, k, lse, w, kv_lens=_i32(*lens))
+    for b in range(B):  # a sequence at a time: the scores of all in 64 bits would not fit
+        want, tol = plain.weigh(q[b:b + 1], k[b:b + 1], lse[b:b + 1], lens[b:b + 1])
+        off = (w[b].double() - before[b].double() - want[0]).abs()
+        assert (off <= tol[0] + 2 * plain.U_F32 * (1 + want[0])).all(), (b, off.max().item())
+        assert torch.equal(w[b, :, lens[b]:], before[b, :, lens[b]:])
+    from rustorch_b200 import _lib
+    assert _lib.device_status() == 0
+
+
+# ------------------------------------------------------------------------------------------------ eviction
+
+
+@pytest.mark.parametrize("B,Hkv,S,keep,recent", [
+    (1, 1, 300_000, 20_000, 100),   # runs of 37,500 in clusters of 8: more than a CTA's shared memory holds
+    (10, 8, 40_000, 3000, 64),      # a CTA each, of up to 39,936 candidates
+    (37, 2, 9000, 500, 7),          # clusters of 2
+    (37, 1, 9000, 8000, 0),         # clusters of 4
+    (9, 2, 40_000, 39_000, 38_000)  # clusters of 8, nearly all kept
+])
+def test_evict_of_long_runs(rt, B, Hkv, S, keep, recent):
+    """Runs that do not fit shared memory beside short ones, and every size of cluster; a third of the weights are equal."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    w = torch.randn(B, Hkv, S, device="cuda", generator=g)
+    w = torch.where(torch.rand(B, Hkv, S, device="cuda", generator=g) < 0.3, 0.25, w)
+    cache = tuple(torch.randint(-9, 9, (B, Hkv, S, 8), device="cuda", generator=g).bfloat16() for _ in "kv")
+    lens = [S if b % 2 == 0 else max(1, keep // 2 if b % 4 == 1 else S - 17 * b) for b in range(B)]
+    out = tuple(torch.full((B, Hkv, keep + 5, 8), 99.0, dtype=torch.bfloat16, device="cuda") for _ in "kv")
+    new_lens, w_out, kept = rt.kv_evict(cache, out, w, keep, recent=recent, kv_lens=_i32(*lens))
+    assert new_lens.tolist() == [min(n, keep) for n in lens]
+    for b, n in enumerate(lens):
+        m = min(n, keep)
+        at = torch.arange(m, device="cuda").expand(Hkv, m)
+        if n > keep:
+            heavy = w[b, :, :n - recent].sort(dim=-1, descending=True, stable=True)[1][:, :keep - recent]
+            at = torch.cat([heavy, torch.arange(n - recent, n, device="cuda").expand(Hkv, recent)], -1).sort(-1)[0]
+        assert torch.equal(kept[b, :, :m].long(), at) and (kept[b, :, m:] == -1).all()
+        assert torch.equal(w_out[b, :, :m], w[b].gather(1, at)) and not w_out[b, :, m:].any()
+        for o, c in zip(out, cache):
+            assert torch.equal(o[b, :, :m], c[b].gather(1, at[..., None].expand(Hkv, m, 8))) and (o[b, :, m:] == 99).all()
