@@ -612,9 +612,16 @@ __global__ void __launch_bounds__(kThreads, Shape<D>::kPerSm) kv4_decode_kernel(
 // Short sequences in one launch: a cluster of CTAs is one (sequence, KV head), its warps take the steps in turn, and the
 // results meet in shared memory: the CTA's four warps', then the cluster's CTAs'.  Scores stay there too until the
 // log-sum-exp is known, so that the weights need no launch of their own.  On the device, here and with workers and merge
-// (and weights) launches, 8 heads, D = 128: 1000 tokens 6.0 and 8.4 us (weighed 7.6 and 11.1), 8000 tokens 10.9 and 16.2 (15.8
-// and 19.0), 16,000 tokens 16.4 and 19.4 (24.4 and 21.9); 16 heads, 8000 tokens 13.0 and 15.8 (18.0 and 17.9).  So up to 8
-// steps a warp.
+// (and weights) launches, 8 KV heads, 32 queries:
+//                          D = 64                         D = 128                        D = 256
+//                          plain          weighed         plain          weighed         plain          weighed
+//      1 x  1000 tokens    5.4 |  7.5      7.0 | 10.4     6.4 |  8.7      8.0 | 11.7     8.8 | 11.4     10.1 | 14.1
+//      1 x  8000           9.0 | 14.9     13.7 | 18.0    11.4 | 17.1     16.0 | 20.1    16.9 | 26.3     21.3 | 29.4
+//      1 x 16,000         12.9 | 16.0     21.3 | 19.5    16.5 | 19.1     25.0 | 22.3    25.4 | 24.3     33.8 | 28.0
+//      4 x  8000          12.7 | 15.3     17.7 | 19.1    15.2 | 21.1     20.3 | 24.9    25.2 | 29.3     35.2 | 34.1
+//     18 x  1000           8.1 | 13.8     11.2 | 16.9     9.2 | 15.5     12.5 | 18.8    one CTA an SM: workers
+//     18 x  4000          19.2 | 25.3     workers        21.8 | 32.5     workers        workers
+// So wherever all clusters are resident at once, up to 8 steps a warp, or 16 where no weights are asked for and D is below 256.
 template <int D>
 struct ClusterShape {
     using S = Shape<D>;
@@ -623,7 +630,8 @@ struct ClusterShape {
     static size_t smem(int score_steps, int group) { return S::kSmem + kResults + (size_t)score_steps * kWarps * kStep * group * 4; }
 };
 constexpr size_t kHalfSm = 112 * 1024;              // shared memory with which two CTAs fit an SM
-constexpr int kMostCluster = 8, kClusterTurns = 8;  // CTAs of a cluster, steps of a warp in one
+constexpr int kMostCluster = 8, kWeighedTurns = 8;  // CTAs of a cluster; steps of a warp whose scores are kept
+constexpr int most_turns(int head_dim, bool weighed) { return weighed || head_dim == 256 ? kWeighedTurns : 16; }
 
 // score_steps: steps of a warp at most, where weights are asked for.
 template <int D, bool kTwice>
@@ -894,7 +902,7 @@ cudaError_t cluster_slots(int size, size_t smem, int& slots) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(size, 1024);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = large ? ClusterShape<D>::smem(kClusterTurns, kMaxGroup) : kHalfSm;
+    cfg.dynamicSmemBytes = large ? ClusterShape<D>::smem(kWeighedTurns, kMaxGroup) : kHalfSm;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = size, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
@@ -908,11 +916,11 @@ cudaError_t cluster_slots(int size, size_t smem, int& slots) {
 // The largest cluster that all groups can have at once and whose warps have a step each at least; 0: none, or too many steps.
 template <int D, bool kTwice>
 cudaError_t pick_cluster(int64_t groups, int64_t steps, bool weighed, int group, int& cluster, int& turns, size_t& smem) {
-    const cudaError_t at = set_max_dynamic_smem_once<kv4_cluster_kernel<D, kTwice>>((int)std::max(ClusterShape<D>::smem(kClusterTurns, kMaxGroup), kHalfSm));
+    const cudaError_t at = set_max_dynamic_smem_once<kv4_cluster_kernel<D, kTwice>>((int)std::max(ClusterShape<D>::smem(kWeighedTurns, kMaxGroup), kHalfSm));
     if (at != cudaSuccess) return at;
     for (cluster = kMostCluster; cluster > 1; cluster /= 2) {
         turns = (int)((steps + cluster * kWarps - 1) / (cluster * kWarps));
-        if (turns > kClusterTurns) break;  // smaller clusters have more
+        if (turns > most_turns(D, weighed)) break;  // smaller clusters have more
         if (steps < cluster * kWarps) continue;
         smem = ClusterShape<D>::smem(weighed ? turns : 0, group);
         int slots = 0;
@@ -965,7 +973,7 @@ cudaError_t launch_kv4_decode(const Kv4Cache& c, const void* q, void* out, float
     p.lse = lse;
     // One launch where all clusters are resident at once and a warp has few steps.
     const int64_t groups = batch * n_kv, longest = kv_lens ? max_seq : kv_len_uniform, steps = (longest + kStep - 1) / kStep;
-    if (steps <= (int64_t)kMostCluster * kWarps * kClusterTurns && groups <= sm_count() / 2) {
+    if (steps <= (int64_t)kMostCluster * kWarps * most_turns(head_dim, weights != nullptr) && groups <= sm_count()) {
         int cluster = 0, turns = 0;
         size_t smem = 0;
         const cudaError_t e = for_form(head_dim, p.group, [&](auto d, auto t) {
@@ -997,7 +1005,9 @@ cudaError_t launch_kv4_decode(const Kv4Cache& c, const void* q, void* out, float
         if (e != cudaSuccess) return e;
         e = launch_chained(kv4_decode_kernel<D, kTwice>, dim3((p.workers + kWarps - 1) / kWarps), kThreads, Shape<D>::kSmem, stream, p);
         if (e == cudaSuccess && p.workers > 1) {
-            // a row has about workers * group / rows parts
+            // A row has about workers * group / rows parts: a CTA a row from 8 on.  The whole call with a CTA a row and a warp a row,
+            // D = 128: 32 rows of 20,000 tokens (222 parts) 19.9 and 69.0 us, 128 of 20,000 (56) 31.2 and 43.9, 512 of 4000 (14)
+            // 30.6 and 32.4, 1024 of 4000 (7) 43.1 and 43.1.
             const int64_t n = batch * n_heads;
             e = p.workers * (int64_t)p.group >= 8 * n
                     ? launch_chained(kv4_merge_kernel<D, true>, dim3((unsigned)n), 32 * kMergeWarps, 0, stream, p)

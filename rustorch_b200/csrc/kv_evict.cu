@@ -225,8 +225,9 @@ cudaError_t launch_kv_evict(const EvictPlanes& planes, const float* weights, flo
     s.weights = weights, s.weights_out = weights_out, s.kept = kept, s.lens_out = lens_out;
     s.max_seq = max_seq, s.max_seq_out = max_seq_out, s.kv_lens = kv_lens, s.kv_len = (int)kv_len_uniform;
     s.n_kv = n_kv, s.keep = (int)keep, s.recent = (int)recent;
-    // More CTAs a head while each keeps 2048 candidates and all find an SM (29,745 candidates of 8 heads: 28.5 us on the device with
-    // one, 19.2 with four, 19.5 with eight).
+    // More CTAs a head while each keeps 2048 candidates and all find an SM.  Replayed from a graph, rows of 16 bytes: 8 heads of
+    // 131,072 tokens 158 us with one CTA a head, 87.5 with two, 32.8 with four, 26.4 with eight; 30,001: 26.6, 20.3, 17.4 and 18.4;
+    // 9000: 13.8, 13.5 and 13.8.
     const int64_t longest = kv_lens ? max_seq : kv_len_uniform;
     int cluster = 1;
     while (cluster < kMostCluster && longest >= 2 * cluster * 2048 && 2 * cluster * batch * n_kv <= sm_count()) cluster *= 2;

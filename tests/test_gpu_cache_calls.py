@@ -27,7 +27,7 @@ def _randn(*shape, seed=0, scale=1.0):
 # ------------------------------------------------------------------------------------------------ decode
 
 
-# max_seq 8192 is the longest that one launch of clusters takes; 20,000 is cut into runs for the workers
+# 8192 tokens are taken in one launch of clusters; 20,000 are cut into runs for the workers
 @pytest.mark.parametrize("S,n", [(8192, 8192), (20000, 20000)])
 @pytest.mark.parametrize("D,G", [(64, 4), (128, 1), (128, 4), (128, 8), (256, 2)])
 @pytest.mark.parametrize("spread", [1e-4, 3e-4, 1e-3, 1e-2])
@@ -90,9 +90,9 @@ def test_decode_of_queries_with_one_large_value(rt, S, D, G, at, far):
     assert ((out[0].double() - want[0]).abs() <= out_tol[0] + 2 * lost[:, None] * values).all()
 
 
-# Below, what runs in one launch of clusters at the sizes of tests/test_gpu_kv4.py is run where the workers take it: more than 8192
-# rows of cache, or more (sequence, KV head) pairs than half the SMs, and several steps a worker.
-@pytest.mark.parametrize("B,S", [(40, 3000), (1, 60000)])
+# Below, what runs in one launch of clusters at the sizes of tests/test_gpu_kv4.py is run where the workers take it: more than
+# 16,384 rows of cache, or more (sequence, KV head) pairs than SMs, and several steps a worker.
+@pytest.mark.parametrize("B,S", [(80, 3000), (1, 60000)])
 @pytest.mark.parametrize("what", ["far scores", "growing scores", "falling scores", "one token", "large q", "small q", "tiny v", "huge v",
                                   "mixed v", "growing v", "scale"])
 def test_decode_of_wide_ranges_in_runs(rt, what, B, S):
@@ -128,7 +128,7 @@ def test_decode_of_wide_ranges_in_runs(rt, what, B, S):
 
 
 @pytest.mark.parametrize("D", [64, 128, 256])
-@pytest.mark.parametrize("n", [8191, 8192, 8193])
+@pytest.mark.parametrize("n", [8191, 8192, 8193, 16383, 16384, 16385])
 @pytest.mark.parametrize("B", [1, 9])
 def test_decode_on_both_sides_of_the_longest_cluster(rt, B, n, D):
     """Weighed and not, as many rows of cache as tokens, then fewer tokens than the cache has room for.  Weights can change how
@@ -144,14 +144,27 @@ def test_decode_on_both_sides_of_the_longest_cluster(rt, B, n, D):
         _check(weights, w, wt + 2 * plain.U_F32 * (1 + w), "weights")
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,D,S", [(18, 32, 8, 128, 1000), (18, 16, 8, 64, 2000), (148, 8, 1, 128, 4096), (74, 4, 2, 64, 4097)])
+def test_decode_of_as_many_clusters_as_fit(rt, B, Hq, Hkv, D, S):
+    """Clusters of two CTAs, two CTAs an SM."""
+    lens = tuple(S - (53 * b) % S for b in range(B))
+    cache, q = plain.fill(rt, B, Hkv, S, D, 13), _randn(B, Hq, D, seed=14)
+    o, l, w, ot, lt, wt = plain.decode(q, cache, lens)
+    for weights in (None, torch.zeros(B, Hkv, S, device="cuda")):
+        out, lse = rt.kv4_decode(q, cache, kv_lens=_i32(*lens), weights=weights)
+        _check(out, o, ot, "out")
+        _check(lse, l, lt, "lse")
+    _check(weights, w, wt + 2 * plain.U_F32 * (1 + w), "weights")
+
+
 @pytest.mark.parametrize("D,Hq,Hkv", [(64, 8, 8), (128, 32, 8), (256, 8, 1)])
 def test_decode_of_a_cache_much_larger_than_its_sequences(rt, D, Hq, Hkv):
     _decode_case(rt, 3, Hq, Hkv, D, 131072, (1000, 33, 257), seed=3)
 
 
 def test_decode_in_runs_does_not_read_rows_behind_the_length(rt):
-    lens = tuple(100 + 37 * b for b in range(45))
-    cache, q = plain.fill(rt, 45, 2, 2000, 128, 5), _randn(45, 8, 128, seed=6)
+    lens = tuple(100 + 23 * b for b in range(80))
+    cache, q = plain.fill(rt, 80, 2, 2000, 128, 5), _randn(80, 8, 128, seed=6)
     want = rt.kv4_decode(q, cache, kv_lens=_i32(*lens))
     for b, n in enumerate(lens):
         cache[1][b, :, n:], cache[3][b, :, n:] = math.nan, math.inf
@@ -159,7 +172,7 @@ def test_decode_in_runs_does_not_read_rows_behind_the_length(rt):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
-@pytest.mark.parametrize("B,S", [(40, 3000), (2, 20001)])
+@pytest.mark.parametrize("B,S", [(80, 3000), (2, 20001)])
 def test_decode_in_runs_keeps_to_its_workspace(rt, B, S):
     """Scratch of exactly the size that is asked for, full of ones: the bytes around it stay."""
     Hq, Hkv, D = 8, 2, 64
@@ -180,7 +193,7 @@ def test_decode_in_runs_keeps_to_its_workspace(rt, B, S):
             _check(weights, w, wt + 2 * plain.U_F32 * (1 + w), "weights")
 
 
-@pytest.mark.parametrize("B,S", [(40, 3000), (2, 20001)])
+@pytest.mark.parametrize("B,S", [(80, 3000), (2, 20001)])
 def test_decode_in_runs_on_streams_and_in_graphs(rt, B, S):
     """Two streams at once, and two graphs that share a pool, replayed with lengths that change: decode, merge and weights."""
     Hq, Hkv, D = 8, 2, 128
