@@ -38,6 +38,11 @@ inline cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, int thre
     return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// CTAs of a (sequence, KV head) whose lengths only the device knows, for a launch whose CTAs walk over what there is: one for each
+// of `most` pieces of the longest, but no more than `per_sm` an SM of all heads together, since the cache may be much larger than
+// what it holds and a CTA without work takes 0.5 to 1 ns of the launch.
+int64_t bounded_blocks(int64_t most, int64_t groups, int per_sm);
+
 // ---- kv4_rows.cu
 cudaError_t launch_kv4_append(const Kv4Cache& c, const void* k, const void* v, const int64_t* ks, const int64_t* vs,
                               int64_t batch, int n_kv, int64_t rows, int head_dim, int64_t max_seq, int64_t pos,

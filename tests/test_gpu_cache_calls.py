@@ -162,6 +162,19 @@ def test_decode_of_a_cache_much_larger_than_its_sequences(rt, D, Hq, Hkv):
     _decode_case(rt, 3, Hq, Hkv, D, 131072, (1000, 33, 257), seed=3)
 
 
+@pytest.mark.parametrize("S", [6000, 6001])
+def test_decode_weights_of_more_tokens_than_a_wave_of_ctas(rt, S):
+    """Weights of 640 (sequence, KV head) pairs: threads that walk over several pieces; rows of weights on 16 bytes and not."""
+    B, Hq, Hkv, D = 160, 8, 4, 64
+    lens = tuple((S - 43 * b) % (S + 1) for b in range(B))
+    cache, q, weights = plain.fill(rt, B, Hkv, S, D, 3), _randn(B, Hq, D, seed=4), torch.zeros(B, Hkv, S, device="cuda")
+    out, lse = rt.kv4_decode(q, cache, kv_lens=_i32(*lens), weights=weights)
+    o, l, w, ot, lt, wt = plain.decode(q, cache, lens)
+    _check(out, o, ot, "out")
+    _check(lse, l, lt, "lse")
+    _check(weights, w, wt + 2 * plain.U_F32 * (1 + w), "weights")
+
+
 def test_decode_in_runs_does_not_read_rows_behind_the_length(rt):
     lens = tuple(100 + 23 * b for b in range(80))
     cache, q = plain.fill(rt, 80, 2, 2000, 128, 5), _randn(80, 8, 128, seed=6)
@@ -269,6 +282,23 @@ def test_weigh_of_rows_that_saw_nothing(rt, T, D, junk):
     else:
         rt.kv_weigh(bad, k, lse, w, kv_lens=_i32(*lens))
     assert ((w.double() - want).abs() <= tol + 2 * plain.U_F32 * (1 + want)).all()
+
+
+@pytest.mark.parametrize("T", [1, 3])
+@pytest.mark.parametrize("B,Hkv,D,S", [(64, 8, 128, 3000), (70, 8, 64, 1500), (64, 8, 256, 1000), (1, 8, 128, 131072)])
+def test_weigh_of_more_tokens_than_a_wave_of_ctas(rt, B, Hkv, D, S, T):
+    """CTAs that walk over several pieces of a sequence, and ones that find none."""
+    G, lens = 2, tuple((S - 37 * b) % S + 1 for b in range(B))
+    q, k = _randn(B, G * Hkv, T, D, seed=1), _randn(B, Hkv, S, D, seed=2)
+    lse = 6 + torch.rand(B, G * Hkv, T, device="cuda")
+    w = torch.zeros(B, Hkv, S, device="cuda")
+    if T == 1:
+        rt.kv_weigh(q[:, :, 0], k, lse[:, :, 0], w, kv_lens=_i32(*lens))
+    else:
+        rt.kv_weigh(q, k, lse, w, kv_lens=_i32(*lens))
+    for b in range(B):
+        want, tol = plain.weigh(q[b:b + 1], k[b:b + 1], lse[b:b + 1], lens[b:b + 1])
+        assert ((w[b].double() - want[0]).abs() <= tol[0] + 2 * plain.U_F32 * (1 + want[0])).all(), b
 
 
 # 296 CTAs at most (148 at D = 256) share the tiles of 128 tokens: here the longest sequences have 4 to 10 for each.  1, 4, 5 and
