@@ -19,10 +19,14 @@ namespace rt {
 namespace {
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-// Query rows of a KV head from which kv_weigh_tc.cu's kernel is taken.  8 heads of 16,001 tokens, here and there: D = 128, 32
-// rows 10.4 and 9.5 us, 64 rows 13.1 and 8.7, 128 rows 20.6 and 12.8; D = 64, 32 rows 8.1 and 8.5 (16 x 2000 tokens: 11.9 and
-// 16.2), 64 rows 10.6 and 8.1; D = 256, 32 rows 22.9 and 15.8.
-__host__ __device__ constexpr int tensor_rows(int head_dim) { return head_dim == 64 ? 64 : 32; }
+// Query rows of a KV head from which kv_weigh_tc.cu's kernel is taken.  Its time hardly depends on their number up to 64.  Here and
+// there, us, 8 heads of 16,001 tokens, 128 of 2000 and 128 of 8000:
+//     D = 64    32 rows  6.3 |  8.1   10.6 | 12.7    37.0 |  50.6     48 rows   7.6 |  8.2   13.1 | 12.8    45.5 |  50.7
+//     D = 128    8 rows  7.1 |  8.8   12.2 | 13.7    48.4 |  56.5     16 rows   8.3 |  8.8   14.4 | 13.8    55.0 |  56.2
+//     D = 256   16 rows 16.7 | 13.4   34.5 | 35.3    96.2 | 121.3     24 rows  19.3 | 13.4   39.2 | 35.3   108.2 | 121.5
+// (60 rows at D = 64: 9.0 | 8.2, 15.4 | 12.8, 54.1 | 50.6.)  Below, a warp loads its keys and then takes the rows: 28 rows at
+// D = 128 waited for the loads half of the time, at 0.4 of the issue rate and 42 % of DRAM's.
+__host__ __device__ constexpr int tensor_rows(int head_dim) { return head_dim == 64 ? 48 : head_dim == 128 ? 16 : 24; }
 
 struct WeighParams {
     const __nv_bfloat16 *q, *k;
@@ -73,7 +77,8 @@ __global__ void __launch_bounds__(kThreads) kv_weigh_kernel(const WeighParams p)
     if ((int)blockIdx.x >= tiles) return;
     const int64_t row0 = bh * p.group * p.seq_q;
     // the query rows: one query's in registers, more in shared memory
-    constexpr int kRows = kSingle ? 8 : tensor_rows(D);  // more than there are
+    constexpr int kRows = kSingle ? 8 : tensor_rows(D);  // as many at least
+    static_assert(kRows % 8 == 0, "rows pass by in eights");
     const int rows = p.group * (int)p.seq_q;
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(8) float s_lse[kRows];

@@ -262,7 +262,7 @@ def test_read_into_tensors_of_the_caller(rt):
 # ------------------------------------------------------------------------------------------------ weights
 
 
-@pytest.mark.parametrize("T,D", [(1, 64), (1, 128), (1, 256), (5, 64), (5, 128), (7, 256), (40, 64), (40, 128), (64, 256), (150, 128)])
+@pytest.mark.parametrize("T,D", [(1, 64), (1, 128), (1, 256), (5, 64), (3, 128), (5, 256), (5, 128), (7, 256), (40, 64), (40, 128), (64, 256), (150, 128)])
 @pytest.mark.parametrize("junk", [math.nan, math.inf])
 def test_weigh_of_rows_that_saw_nothing(rt, T, D, junk):
     """A row whose lse is -inf adds nothing, whatever its query holds: the rows of a batch's padding."""
@@ -285,7 +285,7 @@ def test_weigh_of_rows_that_saw_nothing(rt, T, D, junk):
 
 
 @pytest.mark.parametrize("T", [1, 3])
-@pytest.mark.parametrize("B,Hkv,D,S", [(64, 8, 128, 3000), (70, 8, 64, 1500), (64, 8, 256, 1000), (1, 8, 128, 131072)])
+@pytest.mark.parametrize("B,Hkv,D,S", [(64, 8, 128, 3000), (70, 8, 64, 4000), (64, 8, 256, 1000), (1, 8, 128, 131072)])
 def test_weigh_of_more_tokens_than_a_wave_of_ctas(rt, B, Hkv, D, S, T):
     """CTAs that walk over several pieces of a sequence, and ones that find none."""
     G, lens = 2, tuple((S - 37 * b) % S + 1 for b in range(B))
