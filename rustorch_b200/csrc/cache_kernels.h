@@ -5,6 +5,8 @@
 
 #include <type_traits>
 
+#include "launch_chained.h"
+
 namespace rt {
 
 struct Kv4Cache {
@@ -18,24 +20,6 @@ inline cudaError_t for_head_dim(int head_dim, F&& f) {
         case 128: return f(std::integral_constant<int, 128>{});
         default: return f(std::integral_constant<int, 256>{});
     }
-}
-
-// Launch with programmatic stream serialisation: the kernel may be resident before the one ahead of it in the stream has
-// ended, and waits for it on the device (griddepcontrol.wait) before it touches global memory.
-template <class... Params, class... Args>
-inline cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
-                                  const Args&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 // CTAs of a (sequence, KV head) whose lengths only the device knows, for a launch whose CTAs walk over what there is: one for each

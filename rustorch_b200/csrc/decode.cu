@@ -22,6 +22,7 @@
 #include <algorithm>
 
 #include "kernels.h"
+#include "launch_chained.h"
 
 namespace rt {
 
@@ -710,23 +711,6 @@ __global__ void rope_kv_append_kernel(__nv_bfloat16* q, const __nv_bfloat16* k_i
     }
 }
 
-// Launch with programmatic stream serialisation (the kernel waits for the one before it on the device): a token
-// loop's kernels then overlap their launch latency and set-up with the end of the kernel ahead, and the launch itself
-// costs the host 1.9 us instead of 2.5.
-template <class... Params, class... Args>
-static cudaError_t launch_chained(void (*kernel)(Params...), dim3 grid, int threads, cudaStream_t stream, Args... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3((unsigned)threads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 cudaError_t launch_rope_kv_append(void* q, const void* k_in, const void* v_in, void* k_cache, void* v_cache,
                                   const float* inv_freq, const int32_t* positions, int64_t pos_uniform,
                                   int64_t batch, int n_heads, int n_kv, int head_dim, int64_t max_seq, int style,
@@ -735,7 +719,7 @@ cudaError_t launch_rope_kv_append(void* q, const void* k_in, const void* v_in, v
     dim3 grid(n_heads + n_kv, (unsigned)batch);
     int threads = head_dim / 2;
     threads = threads < 32 ? 32 : (threads > 128 ? 128 : threads);
-    return launch_chained(rope_kv_append_kernel, grid, threads, stream, (__nv_bfloat16*)q, (const __nv_bfloat16*)k_in,
+    return launch_chained(rope_kv_append_kernel, grid, threads, 0, stream, (__nv_bfloat16*)q, (const __nv_bfloat16*)k_in,
                           (const __nv_bfloat16*)v_in, (__nv_bfloat16*)k_cache, (__nv_bfloat16*)v_cache, inv_freq, positions,
                           pos_uniform, n_heads, n_kv, head_dim, max_seq, style);
 }
@@ -1163,7 +1147,7 @@ cudaError_t launch_kv_append(void* k_cache, void* v_cache, const void* k_in, con
                              cudaStream_t stream) {
     if (batch == 0 || n_kv == 0) return cudaSuccess;
     dim3 grid(n_kv, (unsigned)batch);
-    return launch_chained(kv_append_kernel, grid, 64, stream, (__nv_bfloat16*)k_cache, (__nv_bfloat16*)v_cache,
+    return launch_chained(kv_append_kernel, grid, 64, 0, stream, (__nv_bfloat16*)k_cache, (__nv_bfloat16*)v_cache,
                           (const __nv_bfloat16*)k_in, (const __nv_bfloat16*)v_in, n_kv, head_dim, max_seq, pos, positions);
 }
 
