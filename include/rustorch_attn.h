@@ -533,7 +533,7 @@ int rt_kv4_read(const void* k_codes, const void* k_scales, const void* v_codes, 
                 void* v_out, int64_t batch, int n_kv, int head_dim, int64_t max_seq, int64_t rows, int64_t start,
                 const int32_t* starts, const int32_t* kv_lens, void* stream);
 
-/* Bytes of device scratch that rt_kv4_decode needs (weighed: with `weights`). */
+/* Bytes of device scratch that rt_kv4_decode needs (weighed: with `weights`; 4 * B * Hq * max_seq of them hold scores). */
 size_t rt_kv4_decode_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int head_dim, int64_t max_seq,
                                      int weighed);
 

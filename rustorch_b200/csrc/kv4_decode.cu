@@ -118,7 +118,8 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t rest_half2(uint32_t a, uint32_t b, uint32_t ab) {  // a b - ab
-    const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b), __hneg2(*reinterpret_cast<const __half2*>(&ab)));
+    const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                              __hneg2(*reinterpret_cast<const __half2*>(&ab)));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
@@ -324,7 +325,8 @@ __device__ __forceinline__ void step(const uint8_t* stage, int valid, const Quer
     bool larger = false;
 #pragma unroll
     for (int s = 0; s < S::kSpans; ++s) {
-        const uint32_t m = S::kSpans == 2 ? max_half2(max_half2(vw[0][s], vw[0][2 + s]), max_half2(vw[S::kSpans - 1][s], vw[S::kSpans - 1][2 + s]))
+        constexpr int kLast = S::kSpans - 1;
+        const uint32_t m = S::kSpans == 2 ? max_half2(max_half2(vw[0][s], vw[0][2 + s]), max_half2(vw[kLast][s], vw[kLast][2 + s]))
                                           : max_half2(max_half2(vw[0][0], vw[0][1]), max_half2(vw[0][2], vw[0][3]));
         big[s] = max(m & 0xffffu, m >> 16);
         larger |= big[s] > a.scale_limit[s];

@@ -30,7 +30,8 @@ def kv_weigh(q, k_cache, lse, weights, kv_lens=None, kv_len: Optional[int] = Non
     """Adds the softmax weights of q over a bf16 cache to ``weights`` f32 ``[B,Hkv,max_seq]`` (``rt_kv_weigh_bf16``).
 
     q ``[B,Hq,D]``: single-token queries, lse ``[B,Hq]`` as ``gqa_decode`` returned it for them.  Or q ``[B,Hq,T,D]``, lse
-    ``[B,Hq,T]`` from ``prefill_bf16``: the last T tokens of a prompt, each of which sees the tokens up to itself.  k_cache
+    ``[B,Hq,T]`` from ``prefill_bf16``: the last T tokens of a prompt, each of which sees the tokens up to itself (of a padded batch,
+    gathered: they end at ``kv_lens``); a row with lse = -inf adds nothing.  k_cache
     ``[B,Hkv,max_seq,D]`` bf16 (D 64, 128 or 256); ``kv_lens`` int32 CUDA ``[B]`` or a uniform ``kv_len``."""
     if (_lib._binding or _lib.torch_binding()).kv_weigh(q, k_cache, lse, weights, kv_lens, kv_len, scale):
         return
@@ -57,8 +58,8 @@ def kv_evict(cache, out, weights, keep: int, recent: int = 0, kv_lens=None, kv_l
     (``rt_kv_evict``).
 
     ``cache`` and ``out``: two ``Kv4Cache``, or two pairs (k_cache, v_cache) of bf16 ``[B,Hkv,max_seq,D]`` tensors; ``out`` holds
-    at least ``keep`` rows, shares no memory with ``cache`` nor one of its tensors with another, and has its other rows left as they were.  ``weights`` f32
-    ``[B,Hkv,max_seq]``.  Returns (lens int32 ``[B]``, the lengths in ``out``; weights_out f32 ``[B,Hkv,max_seq of out]``, the
+    at least ``keep`` rows, shares no memory with ``cache`` nor one of its tensors with another, and has its other rows left as
+    they were.  ``weights`` f32 ``[B,Hkv,max_seq]``.  Returns (lens int32 ``[B]``, the lengths in ``out``; weights_out f32 ``[B,Hkv,max_seq of out]``, the
     rows' weights, zero behind them; kept int32 ``[B,Hkv,keep]``, the rows' places in ``cache``, -1 behind them)."""
     if type(cache) is type(out) and type(cache) in (Kv4Cache, tuple):
         r = (_lib._binding or _lib.torch_binding()).kv_evict(cache, out, weights, keep, recent, kv_lens, kv_len, weights_out)
