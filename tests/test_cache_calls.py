@@ -1,4 +1,4 @@
-"""Calls of the 4-bit cache and of eviction that need no GPU to be judged: refusals, and rules that the kernels' sources keep."""
+"""Calls of the 4-bit cache and of eviction whose outcome needs no GPU: refusals, and rules that the kernels' sources keep."""
 import glob
 import os
 import re
